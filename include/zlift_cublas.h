@@ -170,8 +170,9 @@ ZLIFT_API cublasStatus_t zlift_sgemm_noalloc(cublasHandle_t handle, int transa, 
 
 /* Returns and clears the device error word: 0 if no kernel of this library
  * has recorded an error on the current device since the last call,
- * otherwise 1 (a bounded device-side wait timed out).  Synchronises the
- * current device. */
+ * otherwise 1 (a bounded device-side wait timed out) or 2 (a paged-cache
+ * call met a page, slot or length outside its bounds and did not follow it).
+ * Synchronises the current device. */
 ZLIFT_API int zlift_device_error(void);
 
 /* Number of kernels this library launched on any stream since load. */

@@ -95,6 +95,11 @@ SIGNATURES = [
     ("zlift_part_register_peer_buffer", c_int, [c_void_p, c_int, c_int, c_void_p, c_size_t]),
     ("zlift_part_unregister_peer_buffer", c_int, [c_void_p, c_void_p]),
     ("zlift_part_flash_fwd", c_int, [c_void_p, c_uint, c_int, c_ll, c_ll, c_void_p]),
+    ("zlift_kv_write", c_int, [c_void_p, c_void_p, c_void_p, c_void_p]),
+    ("zlift_kv_read", c_int, [c_void_p, c_void_p, c_void_p, c_ll, c_int, c_void_p, c_void_p,
+                              c_int, c_void_p]),
+    ("zlift_paged_attn_workspace", c_size_t, [c_void_p, c_void_p]),
+    ("zlift_paged_attn", c_int, [c_void_p, c_void_p, c_void_p]),
 ]
 
 
@@ -121,6 +126,8 @@ def load(path: str | None = None) -> ctypes.CDLL:
 
 from .blas import Handle, GemmError  # noqa: E402
 from .attention import flash_forward, fmha_forward, FlashParams, FmhaParams  # noqa: E402
+from .paged import KVCache, kv_write, kv_read, paged_attention  # noqa: E402
 
 __all__ = ["load", "Handle", "GemmError", "flash_forward", "fmha_forward",
-           "FlashParams", "FmhaParams", "LIBCUBLAS", "LIBCUDNN"]
+           "FlashParams", "FmhaParams", "KVCache", "kv_write", "kv_read", "paged_attention",
+           "LIBCUBLAS", "LIBCUDNN"]

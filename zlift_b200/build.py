@@ -34,7 +34,8 @@ NVCC_FLAGS = ARCH + [
     "-I", os.path.join(ROOT, "include"),
 ]
 # kernels whose arithmetic must not be relaxed by --use_fast_math
-PRECISE = {"gemm_simt.cu", "gemm_tc.cu", "cublas_api.cu", "attn_f32.cu"}
+PRECISE = {"gemm_simt.cu", "gemm_tc.cu", "cublas_api.cu", "attn_f32.cu", "kv_cache.cu",
+           "paged_simt.cu"}
 
 SOURCES = [
     "gemm_tc.cu",
@@ -45,6 +46,9 @@ SOURCES = [
     "cublas_api.cu",
     "partition.cu",
     "noalloc.cu",
+    "kv_cache.cu",
+    "paged_simt.cu",
+    "paged_api.cu",
 ]
 
 

@@ -785,7 +785,11 @@ int zlift_device_error(void) {
     int e2 = gemm_simt_error(true);
     int e3 = fmha_error(true);
     int e4 = part_error(true);
-    return e ? e : (e2 ? e2 : (e3 ? e3 : e4));
+    int e5 = kv_cache_error(true);
+    int e6 = paged_simt_error(true);
+    for (int v : {e, e2, e3, e4, e5, e6})
+        if (v) return v;
+    return 0;
 }
 
 unsigned long long zlift_launch_count(void) { return launch_count(); }

@@ -133,6 +133,8 @@ unsigned long long wait_limit_ns();
 int wait_probe(unsigned long long limit_ns, cudaStream_t s);
 int gemm_simt_error(bool clear);
 int fmha_error(bool clear);
+int kv_cache_error(bool clear);
+int paged_simt_error(bool clear);
 
 // Trace switch (ZBLAS_TRACE set in the environment).
 bool tracing();
