@@ -787,7 +787,8 @@ int zlift_device_error(void) {
     int e4 = part_error(true);
     int e5 = kv_cache_error(true);
     int e6 = paged_simt_error(true);
-    for (int v : {e, e2, e3, e4, e5, e6})
+    int e7 = paged_decode_error(true);
+    for (int v : {e, e2, e3, e4, e5, e6, e7})
         if (v) return v;
     return 0;
 }

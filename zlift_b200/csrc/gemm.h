@@ -135,6 +135,7 @@ int gemm_simt_error(bool clear);
 int fmha_error(bool clear);
 int kv_cache_error(bool clear);
 int paged_simt_error(bool clear);
+int paged_decode_error(bool clear);
 
 // Trace switch (ZBLAS_TRACE set in the environment).
 bool tracing();

@@ -105,5 +105,8 @@ int kv_read(const KvView& c, int type, const zlift_kv_rows& r, const int* table,
             long long tstride, int tpages, const int* starts, const int* cu, int batch,
             cudaStream_t s);
 int paged_attn_simt(const PagedAttn& a, cudaStream_t s);
+int paged_decode(const PagedAttn& a, cudaStream_t s);
+int decode_blocks();
+size_t paged_decode_workspace(const PagedAttn& a);
 
 }  // namespace zl

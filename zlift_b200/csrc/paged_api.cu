@@ -60,7 +60,8 @@ bool describe(const zlift_kv_cache* cache, const zlift_paged_attn_params* p, Pag
     if (a.c.dim > 256) return no("dim above 256");
     if (p->batch < 0 || p->total_q < 0 || p->table_pages < 0) return no("negative size");
     if (p->heads <= 0 || p->heads > 65535 || p->heads % a.c.heads) return no("head grouping");
-    if ((long long)p->table_pages * a.c.ps > 0x7fffffffLL) return no("2^31 keys in a sequence");
+    // (some room below 2^31, so that key numbers a few tiles past the end fit)
+    if ((long long)p->table_pages * a.c.ps > 0x7fff0000LL) return no("2^31 keys in a sequence");
     if (p->batch > 0 && p->total_q > 0 &&
         (!p->q || !p->o || !p->cu_q || !p->seq_k || (!p->page_table && p->table_pages > 0)))
         return no("null operand");
@@ -80,6 +81,33 @@ bool describe(const zlift_kv_cache* cache, const zlift_paged_attn_params* p, Pag
     a.ws_bytes = p->workspace_bytes;
     a.elem = p->elem; a.type = cache->type;
     return true;
+}
+
+enum class Way { Simt, Decode };
+
+// Which kernel serves a call.  The tensor-core kernels take rows in 16-byte
+// pieces, find a token by a 32-bit count of 32 bytes, and scale by a positive
+// factor after the running maximum.
+Way choose(const PagedAttn& a) {
+    const int eb = a.type >= kI8 ? 1 : 2;
+    if (a.c.dim != 64 && a.c.dim != 128) return Way::Simt;
+    if (!(a.scale > 0.f) || !std::isfinite(a.scale)) return Way::Simt;
+    if (a.c.page < 0 || a.c.row < 0 || a.c.head < 0) return Way::Simt;
+    if ((a.c.page * eb) % 32 || (a.c.row * eb) % 32 || (a.c.head * eb) % 16) return Way::Simt;
+    const double span = ((double)(a.c.pages - 1) * a.c.page + (double)(a.c.ps - 1) * a.c.row) * eb;
+    if (span / 32 >= 4294967295.0) return Way::Simt;
+    if ((a.qr * 2) % 16 || (a.qh * 2) % 16) return Way::Simt;
+    for (const void* p : {(const void*)a.q, (const void*)a.c.k, (const void*)a.c.v})
+        if (reinterpret_cast<uintptr_t>(p) & 15u) return Way::Simt;
+    if (a.group > 16) return Way::Simt;
+    return Way::Decode;
+}
+
+size_t workspace_of(const PagedAttn& a) {
+    switch (choose(a)) {
+    case Way::Decode: return paged_decode_workspace(a);
+    default: return 0;
+    }
 }
 
 }  // namespace
@@ -125,14 +153,22 @@ int zlift_kv_read(const zlift_kv_cache* cache, const zlift_kv_rows* rows,
 size_t zlift_paged_attn_workspace(const zlift_kv_cache* cache, const zlift_paged_attn_params* p) {
     PagedAttn a;
     if (!describe(cache, p, a)) return 0;
-    return 0;
+    return workspace_of(a);
 }
 
 int zlift_paged_attn(const zlift_kv_cache* cache, const zlift_paged_attn_params* p, void* stream) {
     PagedAttn a;
     if (!describe(cache, p, a)) return 1;
     if (a.batch == 0 || a.total_q == 0) return 0;
-    return finish("paged attention", paged_attn_simt(a, static_cast<cudaStream_t>(stream)));
+    const char* who = "paged attention";
+    const size_t need = workspace_of(a);
+    if (need && (!a.ws || a.ws_bytes < need || (reinterpret_cast<uintptr_t>(a.ws) & 255u)))
+        return declined(who, "workspace missing, small or unaligned");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    switch (choose(a)) {
+    case Way::Decode: return finish(who, paged_decode(a, s));
+    default: return finish(who, paged_attn_simt(a, s));
+    }
 }
 
 }  // extern "C"

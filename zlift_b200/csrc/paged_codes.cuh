@@ -1,0 +1,99 @@
+// paged_codes.cuh -- 8-bit cache codes as 16-bit matrix operands, exactly.
+#pragma once
+#include "paged.h"
+
+namespace zl {
+
+// widen(u, lo, hi): the four codes in u as two pairs of 16-bit values (codes 0
+// and 1 in lo, 2 and 3 in hi), each the code's value divided by kUnscale.
+template <int ELEM, int CT>
+struct Code {                            // a 16-bit cache: nothing to widen
+    static constexpr float kUnscale = 1.f;
+};
+
+// int8 -> fp16: 0x6400 | (c + 128) is 1024 + 128 + c
+template <>
+struct Code<kF16, kI8> {
+    static constexpr float kUnscale = 1.f;
+    static __device__ __forceinline__ void widen(uint32_t u, uint32_t& lo, uint32_t& hi) {
+        const uint32_t x = u ^ 0x80808080u;
+        const uint32_t k = 0x64806480u;              // 1152
+        uint32_t a = __byte_perm(x, 0x64646464u, 0x4140), b = __byte_perm(x, 0x64646464u, 0x4342);
+        const __half2 kh = *reinterpret_cast<const __half2*>(&k);
+        const __half2 ah = __hsub2(*reinterpret_cast<__half2*>(&a), kh);
+        const __half2 bh = __hsub2(*reinterpret_cast<__half2*>(&b), kh);
+        lo = *reinterpret_cast<const uint32_t*>(&ah);
+        hi = *reinterpret_cast<const uint32_t*>(&bh);
+    }
+};
+
+// int8 -> bf16, whose 8 significant bits hold no offset of 128 beside 8 bits:
+// with c = low7 - 128 * sign, (128 + low7) - (128 or 256, by the sign) = c
+template <>
+struct Code<kBF16, kI8> {
+    static constexpr float kUnscale = 1.f;
+    static __device__ __forceinline__ uint32_t half(uint32_t y) {   // bytes c, 0x43, c, 0x43
+        uint32_t a = y & 0xff7fff7fu, b = y & 0xff80ff80u;
+        const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a),
+                                         *reinterpret_cast<__nv_bfloat162*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+    static __device__ __forceinline__ void widen(uint32_t u, uint32_t& lo, uint32_t& hi) {
+        lo = half(__byte_perm(u, 0x43434343u, 0x4140));
+        hi = half(__byte_perm(u, 0x43434343u, 0x4342));
+    }
+};
+
+// e4m3 -> fp16: sign, 4 exponent and 3 mantissa bits moved into place; the
+// exponent bias differs by 8, so the value is 2^-8 of the code's, subnormal
+// codes included (fp16's own subnormals hold them).  The caller multiplies
+// the product by kUnscale.
+template <>
+struct Code<kF16, kE4M3> {
+    static constexpr float kUnscale = 256.f;
+    static __device__ __forceinline__ uint32_t half(uint32_t p) {   // codes in the high bytes
+        return (p & 0x80008000u) | ((p >> 1) & 0x3f803f80u);
+    }
+    static __device__ __forceinline__ void widen(uint32_t u, uint32_t& lo, uint32_t& hi) {
+        lo = half(__byte_perm(u, 0u, 0x1404));
+        hi = half(__byte_perm(u, 0u, 0x3424));
+    }
+};
+
+// e4m3 -> bf16: the same, 2^-120 of the code's value; brought back at once,
+// for products that small would leave fp32's normal range
+template <>
+struct Code<kBF16, kE4M3> {
+    static constexpr float kUnscale = 1.f;
+    static __device__ __forceinline__ uint32_t half(uint32_t p) {
+        uint32_t x = (p & 0x80008000u) | ((p >> 4) & 0x07f007f0u);
+        const uint32_t k = 0x7b807b80u;              // 2^120
+        const __nv_bfloat162 r = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&x),
+                                         *reinterpret_cast<const __nv_bfloat162*>(&k));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+    static __device__ __forceinline__ void widen(uint32_t u, uint32_t& lo, uint32_t& hi) {
+        lo = half(__byte_perm(u, 0u, 0x1404));
+        hi = half(__byte_perm(u, 0u, 0x3424));
+    }
+};
+
+// fp16 weights carry a power of two `pow` beside the V scales, so that neither
+// a large scale (up to 516 times a weight of 64) overflows nor a small one
+// loses its bits to fp16's subnormals: pow * (largest scale seen) stays in
+// [1, 512].  Takes the largest scale of the next keys; returns the factor by
+// which the O summed so far has to be multiplied.
+__device__ __forceinline__ float v_power(float big, float& most, float& pow) {
+    if (!(big > most)) return 1.f;
+    most = big;
+    const float x = big * pow;
+    if (x >= 1.f && x <= 512.f) return 1.f;
+    // 2^-exponent(big), kept within what fp32 holds both ways
+    const int e = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 100);
+    const float next = __uint_as_float((uint32_t)(127 - e) << 23);
+    const float fix = next / pow;
+    pow = next;
+    return fix;
+}
+
+}  // namespace zl

@@ -1,0 +1,184 @@
+// paged_sched.cuh -- how a paged-attention launch is split over its blocks.
+//
+// A unit is a tile of query rows of one sequence and KV head; its steps are
+// the key tiles that its rows see (one at least, so that rows which see
+// nothing are written too).  All steps of all units, in the order sequence,
+// head, tile, key, form one line, and block x takes the x-th equal piece of
+// it.  Lengths live on the device, so every block works its piece out from
+// them: nothing is planned on the host, a ragged batch is as even as a
+// regular one, and a graph replays with new lengths.
+//
+// A unit that spans several blocks is joined by whichever of them finishes
+// last: each leaves its unnormalised O with the maximum and the sum of every
+// row in the workspace and counts itself on the unit's counter; the last one
+// sums the parts in key order (so the result does not depend on who came
+// last) and puts the counter back to zero for the next call.  A block has at
+// most two partial units: one that began before its piece (slot 0, also
+// where it ends after it) and one that begins in it (slot 1).  The counter is
+// that of the block in which the unit begins, of which no other unit that
+// begins there runs out.
+#pragma once
+#include "paged.h"
+
+namespace zl {
+
+struct SchedShape {
+    int tokens;          // query tokens per tile
+    int step;            // keys per step
+    int least;           // steps per block, at least
+};
+
+// one block's piece of one unit
+struct Segment {
+    int s, head;         // sequence, KV head
+    SeqInfo q;
+    int i0, ni;          // the tile's first token in the chunk, and tokens
+    int k0, k1;          // its keys in this piece (k1 is not rounded up)
+    int parts, part;     // blocks that share the unit; this block's place
+    int first;           // the block in which the unit begins
+};
+
+__device__ __forceinline__ int tile_end(const PagedAttn& a, const SeqInfo& q, int i1) {
+    return a.causal ? max(0, min(q.len, q.len - q.n + i1)) : q.len;
+}
+
+__device__ __forceinline__ int tile_steps(const PagedAttn& a, const SchedShape& h,
+                                          const SeqInfo& q, int tile) {
+    const int e = tile_end(a, q, min(q.n, (tile + 1) * h.tokens));
+    return max(1, (int)((unsigned)(e + h.step - 1) / (unsigned)h.step));
+}
+
+// steps of all tiles of one head of a sequence
+__device__ __forceinline__ long long head_steps(const PagedAttn& a, const SchedShape& h,
+                                                const SeqInfo& q) {
+    const int tiles = (q.n + h.tokens - 1) / h.tokens;
+    if (!a.causal) return tiles ? (long long)tiles * tile_steps(a, h, q, 0) : 0;
+    long long sum = 0;
+    for (int t = 0; t < tiles; t++) sum += tile_steps(a, h, q, t);
+    return sum;
+}
+
+// Walks a block's piece.  Every warp keeps one of its own (the search runs
+// across the lanes; all lanes hold the same state afterwards).
+struct Walker {
+    long long pos, end, per, begin;      // on the line; begin: of the unit
+    SeqInfo q;
+    int s, head, tile, steps;
+
+    __device__ __forceinline__ void enter(const PagedAttn& a, const SchedShape& h) {
+        steps = tile_steps(a, h, q, tile);
+    }
+
+    __device__ void start(const PagedAttn& a, const SchedShape& h, int block, int blocks) {
+        const int lane = threadIdx.x & 31;
+        long long mine = 0;
+        for (int b = lane; b < a.batch; b += 32) mine += head_steps(a, h, seq_info(a, b));
+        mine *= a.c.heads;
+        long long total = mine;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        per = max((total + blocks - 1) / blocks, (long long)h.least);
+        pos = min(total, block * per);
+        end = min(total, pos + per);
+        if (pos >= end) return;
+        // the sequence that holds pos: running sums over 32 sequences at a time
+        long long base = 0;
+        for (int b0 = 0;; b0 += 32) {
+            const int b = b0 + lane;
+            long long v = a.batch <= 32 ? mine
+                        : b < a.batch ? head_steps(a, h, seq_info(a, b)) * a.c.heads : 0;
+            long long sum = v;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long x = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += x;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, base + sum > pos);
+            if (past) {
+                const int l = __ffs(past) - 1;
+                s = b0 + l;
+                base += __shfl_sync(0xffffffffu, sum - v, l);
+                break;
+            }
+            base += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        q = seq_info(a, s);
+        const long long hs = head_steps(a, h, q);
+        head = (int)((pos - base) / hs);
+        begin = base + head * hs;
+        tile = 0;
+        enter(a, h);
+        while (pos - begin >= steps) {
+            begin += steps;
+            tile++;
+            enter(a, h);
+        }
+    }
+
+    // the next piece of a unit; false at the end of the line's piece
+    __device__ __forceinline__ bool next(const PagedAttn& a, const SchedShape& h, int block,
+                                         Segment& g) {
+        if (pos >= end) return false;
+        g.s = s;
+        g.head = head;
+        g.q = q;
+        g.i0 = tile * h.tokens;
+        g.ni = min(h.tokens, q.n - g.i0);
+        const int st0 = (int)(pos - begin);
+        const int st1 = (int)min((long long)steps, end - begin);
+        const int e = tile_end(a, q, g.i0 + g.ni);
+        g.k0 = min(e, st0 * h.step);
+        g.k1 = (int)min((long long)e, (long long)st1 * h.step);
+        if (st0 == 0 && st1 == steps) {
+            g.parts = 1;
+            g.part = 0;
+            g.first = block;
+        } else {
+            g.first = (int)(begin / per);
+            g.parts = (int)((begin + steps - 1) / per) - g.first + 1;
+            g.part = block - g.first;
+        }
+        pos = begin + st1;
+        if (st1 == steps && pos < end) {
+            begin += steps;
+            if (++tile * h.tokens >= q.n) {
+                tile = 0;
+                if (++head == a.c.heads) {
+                    head = 0;
+                    do q = seq_info(a, ++s);
+                    while (q.n == 0);
+                }
+            }
+            enter(a, h);
+        }
+        return true;
+    }
+};
+
+// ---- the workspace --------------------------------------------------------------
+
+constexpr int kMaxBlocks = 1024;                 // counters: one per block
+constexpr size_t kCounterBytes = kMaxBlocks * sizeof(int);
+
+// floats of one slot: (maximum, sum) of every row, then O
+__host__ __device__ constexpr long long slot_floats(int rows, int dim) {
+    return (long long)rows * (2 + dim);
+}
+
+__device__ __forceinline__ float* part_slot(const PagedAttn& a, int rows, int block, bool begins) {
+    return reinterpret_cast<float*>(a.ws + kCounterBytes) +
+           (2LL * block + (begins ? 1 : 0)) * slot_floats(rows, a.c.dim);
+}
+
+// Called by every thread of a group of `threads` (a __syncthreads group or a
+// named barrier) after its part is stored and the group has synchronised
+// behind a __threadfence(): by one thread, which learns whether the part was
+// the unit's last.
+__device__ __forceinline__ bool count_part(const PagedAttn& a, const Segment& g) {
+    int* counter = reinterpret_cast<int*>(a.ws) + g.first;
+    const bool last = atomicAdd(counter, 1) == g.parts - 1;
+    if (last) atomicExch(counter, 0);
+    return last;
+}
+
+}  // namespace zl

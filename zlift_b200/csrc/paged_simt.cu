@@ -15,7 +15,7 @@ namespace {
 
 constexpr int kWarps = 4;
 
-__global__ void __launch_bounds__(kWarps * 32) paged_attn_simt_kernel(const PagedAttn a) {
+__global__ void __launch_bounds__(kWarps * 32) paged_attn_simt_kernel(const __grid_constant__ PagedAttn a) {
     __shared__ float sm[kWarps], sl[kWarps], sacc[kWarps][32 * kRowCols];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int head = blockIdx.y;

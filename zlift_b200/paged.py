@@ -231,6 +231,7 @@ def attention_workspace(cache: KVCache, heads, total_q, max_q, batch, elem=None)
     p = AttnBlock()
     p.batch, p.total_q, p.max_q, p.heads = batch, total_q, max_q, heads
     p.elem = cache.type if cache.type < I8 else (BF16 if elem is None else elem)
+    p.scale = 1.0
     fake = 256                       # not followed: only sizes are looked at
     p.q = p.o = p.cu_q = p.seq_k = p.page_table = fake
     p.q_row_stride = p.o_row_stride = heads * cache.dim
