@@ -35,7 +35,7 @@ NVCC_FLAGS = ARCH + [
 ]
 # kernels whose arithmetic must not be relaxed by --use_fast_math
 PRECISE = {"gemm_simt.cu", "gemm_tc.cu", "cublas_api.cu", "attn_f32.cu", "kv_cache.cu",
-           "paged_simt.cu", "paged_decode.cu"}
+           "paged_simt.cu", "paged_decode.cu", "paged_chunk.cu"}
 
 SOURCES = [
     "gemm_tc.cu",
@@ -49,6 +49,7 @@ SOURCES = [
     "kv_cache.cu",
     "paged_simt.cu",
     "paged_decode.cu",
+    "paged_chunk.cu",
     "paged_api.cu",
 ]
 

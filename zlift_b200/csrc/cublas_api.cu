@@ -788,7 +788,8 @@ int zlift_device_error(void) {
     int e5 = kv_cache_error(true);
     int e6 = paged_simt_error(true);
     int e7 = paged_decode_error(true);
-    for (int v : {e, e2, e3, e4, e5, e6, e7})
+    int e8 = paged_chunk_error(true);
+    for (int v : {e, e2, e3, e4, e5, e6, e7, e8})
         if (v) return v;
     return 0;
 }
@@ -798,7 +799,8 @@ unsigned long long zlift_launch_count(void) { return launch_count(); }
 int zlift_set_wait_limit_ns(unsigned long long ns) {
     if (ns == 0) return CUBLAS_STATUS_INVALID_VALUE;
     const int r = gemm_tc_set_wait_limit(ns) | gemm_simt_set_wait_limit(ns) |
-                  fmha_set_wait_limit(ns) | part_set_wait_limit(ns);
+                  fmha_set_wait_limit(ns) | part_set_wait_limit(ns) |
+                  paged_chunk_set_wait_limit(ns);
     return r ? CUBLAS_STATUS_EXECUTION_FAILED : CUBLAS_STATUS_SUCCESS;
 }
 

@@ -136,6 +136,8 @@ int fmha_error(bool clear);
 int kv_cache_error(bool clear);
 int paged_simt_error(bool clear);
 int paged_decode_error(bool clear);
+int paged_chunk_error(bool clear);
+int paged_chunk_set_wait_limit(unsigned long long ns);
 
 // Trace switch (ZBLAS_TRACE set in the environment).
 bool tracing();

@@ -108,5 +108,8 @@ int paged_attn_simt(const PagedAttn& a, cudaStream_t s);
 int paged_decode(const PagedAttn& a, cudaStream_t s);
 int decode_blocks();
 size_t paged_decode_workspace(const PagedAttn& a);
+int paged_chunk(const PagedAttn& a, cudaStream_t s);
+int chunk_blocks();
+size_t paged_chunk_workspace(const PagedAttn& a);
 
 }  // namespace zl

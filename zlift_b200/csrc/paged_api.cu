@@ -83,7 +83,7 @@ bool describe(const zlift_kv_cache* cache, const zlift_paged_attn_params* p, Pag
     return true;
 }
 
-enum class Way { Simt, Decode };
+enum class Way { Simt, Decode, Chunk };
 
 // Which kernel serves a call.  The tensor-core kernels take rows in 16-byte
 // pieces, find a token by a 32-bit count of 32 bytes, and scale by a positive
@@ -99,13 +99,23 @@ Way choose(const PagedAttn& a) {
     if ((a.qr * 2) % 16 || (a.qh * 2) % 16) return Way::Simt;
     for (const void* p : {(const void*)a.q, (const void*)a.c.k, (const void*)a.c.v})
         if (reinterpret_cast<uintptr_t>(p) & 15u) return Way::Simt;
-    if (a.group > 16) return Way::Simt;
-    return Way::Decode;
+    // the chunk kernel's boxes: whole ones inside a page (16 bit), queries and
+    // output rows by 16-byte pieces
+    auto steps = [](long long stride, int count) { return stride > 0 || count == 1; };
+    const bool boxes = (a.type >= kI8 || (a.c.ps % 8 == 0 && steps(a.c.row, a.c.ps) &&
+                                          steps(a.c.head, a.c.heads) && steps(a.c.page, a.c.pages))) &&
+                       steps(a.qr, a.total_q) && steps(a.qh, a.heads) &&
+                       a.group <= 128 && (reinterpret_cast<uintptr_t>(a.o) & 15u) == 0 &&
+                       (a.orow * 2) % 16 == 0 && (a.oh * 2) % 16 == 0;
+    const long long rows = (long long)(a.max_q > 1 ? a.max_q : 1) * a.group;
+    if (a.group <= 16 && (rows <= 16 || !boxes)) return Way::Decode;
+    return boxes ? Way::Chunk : Way::Simt;
 }
 
 size_t workspace_of(const PagedAttn& a) {
     switch (choose(a)) {
     case Way::Decode: return paged_decode_workspace(a);
+    case Way::Chunk: return paged_chunk_workspace(a);
     default: return 0;
     }
 }
@@ -167,6 +177,7 @@ int zlift_paged_attn(const zlift_kv_cache* cache, const zlift_paged_attn_params*
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (choose(a)) {
     case Way::Decode: return finish(who, paged_decode(a, s));
+    case Way::Chunk: return finish(who, paged_chunk(a, s));
     default: return finish(who, paged_attn_simt(a, s));
     }
 }

@@ -157,8 +157,8 @@ struct Walker {
 
 // ---- the workspace --------------------------------------------------------------
 
-constexpr int kMaxBlocks = 1024;                 // counters: one per block
-constexpr size_t kCounterBytes = kMaxBlocks * sizeof(int);
+constexpr int kMaxBlocks = 1024;                 // two counters each
+constexpr size_t kCounterBytes = 2 * kMaxBlocks * sizeof(int);
 
 // floats of one slot: (maximum, sum) of every row, then O
 __host__ __device__ constexpr long long slot_floats(int rows, int dim) {
