@@ -106,7 +106,7 @@ int kv_read(const KvView& c, int type, const zlift_kv_rows& r, const int* table,
             cudaStream_t s);
 int paged_attn_simt(const PagedAttn& a, cudaStream_t s);
 int paged_decode(const PagedAttn& a, cudaStream_t s);
-int decode_blocks();
+int decode_max_rows();
 size_t paged_decode_workspace(const PagedAttn& a);
 int paged_chunk(const PagedAttn& a, cudaStream_t s);
 int chunk_blocks();

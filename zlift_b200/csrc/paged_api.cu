@@ -99,16 +99,17 @@ Way choose(const PagedAttn& a) {
     if ((a.qr * 2) % 16 || (a.qh * 2) % 16) return Way::Simt;
     for (const void* p : {(const void*)a.q, (const void*)a.c.k, (const void*)a.c.v})
         if (reinterpret_cast<uintptr_t>(p) & 15u) return Way::Simt;
+    auto steps = [](long long stride, int count) { return stride > 0 || count == 1; };
+    if (a.c.ps % 8 || !steps(a.c.row, a.c.ps) || !steps(a.c.head, a.c.heads) ||
+        !steps(a.c.page, a.c.pages))
+        return Way::Simt;
     // the chunk kernel's boxes: whole ones inside a page (16 bit), queries and
     // output rows by 16-byte pieces
-    auto steps = [](long long stride, int count) { return stride > 0 || count == 1; };
-    const bool boxes = (a.type >= kI8 || (a.c.ps % 8 == 0 && steps(a.c.row, a.c.ps) &&
-                                          steps(a.c.head, a.c.heads) && steps(a.c.page, a.c.pages))) &&
-                       steps(a.qr, a.total_q) && steps(a.qh, a.heads) &&
+    const bool boxes = steps(a.qr, a.total_q) && steps(a.qh, a.heads) &&
                        a.group <= 128 && (reinterpret_cast<uintptr_t>(a.o) & 15u) == 0 &&
                        (a.orow * 2) % 16 == 0 && (a.oh * 2) % 16 == 0;
     const long long rows = (long long)(a.max_q > 1 ? a.max_q : 1) * a.group;
-    if (a.group <= 16 && (rows <= 16 || !boxes)) return Way::Decode;
+    if (a.group <= decode_max_rows() && (rows <= decode_max_rows() || !boxes)) return Way::Decode;
     return boxes ? Way::Chunk : Way::Simt;
 }
 

@@ -47,27 +47,31 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kRows = 16;
-constexpr int kStages = 3;
-constexpr int kBlocksPerSM = 2;
+constexpr int kMaxNB = 3;
 constexpr float kLazy = 6.f;
-constexpr uint32_t kNone = 0xffffffffu;
 constexpr float kLog2e = 1.4426950408889634f;
 
-template <int D, int CT>
+template <int D, int CT, int NB>
 struct DCfg {
     static constexpr int EB = kv_bytes<CT>;
     static constexpr bool Q8 = CT >= kI8;
+    static constexpr int ROWS = 8 * NB;
     static constexpr int BK = 4096 / (D * EB);           // keys per block: 4 KB of K, 4 KB of V
-    static constexpr int NT = BK / 8;                    // score tiles
+    static constexpr int NT = BK / 8;
     static constexpr int KCH = D * EB / 64;              // 16-byte K pieces per lane and key
     static constexpr int VP = D * EB >= 128 ? 16 : 8;    // bytes of a V piece
     static constexpr int VCH = D * EB / (8 * VP);        // V pieces per lane and key
     static constexpr int VE = VP / EB;                   // elements of one
-    static constexpr int STAGE = 8192 + (Q8 ? 2 * BK * 4 : 0) + 16;
-    static constexpr int RING = kStages * STAGE;
-    static constexpr int JOIN = kWarps * kRows * (D + 4) * 4;
-    static constexpr int SMEM = kWarps * RING > JOIN ? kWarps * RING : JOIN;
+    static constexpr int RB = D * EB > 128 ? 128 : D * EB;   // bytes of a row in a box
+    static constexpr int CB = D * EB / RB;               // boxes side by side
+    static constexpr int PER_SM = NB == 1 ? 3 : 2;       // blocks per SM
+    static constexpr int STAGES = NB == 1 ? 2 : 3;
+    static constexpr int RING = STAGES * 8192;
+    static constexpr int SIDE = (Q8 ? 2 * BK * 4 : 0) + 16;  // scales, keys there; per stage
+    static constexpr int SIDE_OFF = kWarps * RING;
+    static constexpr int JOIN = kWarps * ROWS * (D + 4) * 4;
+    static constexpr int SMEM = SIDE_OFF + kWarps * STAGES * SIDE + 1024;
+    static_assert(JOIN <= SIDE_OFF, "the join reuses the rings");
     static_assert(NT * KCH == 8 && BK / 4 * VCH * VP == 128, "a block is 8 KB");
 };
 
@@ -94,30 +98,31 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 
 // 16 x 8 += 16 x 16 . 16 x 8
 template <int ELEM>
-__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
-                                      uint32_t b1) {
+__device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                      uint32_t a3, const uint32_t (&b)[2]) {
     if constexpr (ELEM == kBF16)
         asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
             "{%8,%9}, {%0,%1,%2,%3};"
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]));
     else
         asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
             "{%8,%9}, {%0,%1,%2,%3};"
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]));
 }
 
-// copies N bytes, or writes N zeros where `there` is false (src is not read then)
-template <int N>
-__device__ __forceinline__ void copy_async(uint32_t dst, const char* src, bool there) {
-    const int bytes = there ? N : 0;
-    if constexpr (N == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-                     :: "r"(dst), "l"(src), "r"(bytes) : "memory");
-    else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;"
-                     :: "r"(dst), "l"(src), "r"(bytes), "n"(N) : "memory");
+// an 8 x 8 matrix of 16-bit values across the warp, transposed
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// copies a scale, or writes zero where `there` is false (src is not read then)
+__device__ __forceinline__ void copy_async4(uint32_t dst, const float* src, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;"
+                 :: "r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
 }
 __device__ __forceinline__ void copy_commit() {
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -144,79 +149,58 @@ __device__ __forceinline__ uint32_t lds4(uint32_t a) {
     return v;
 }
 
-template <int D, int ELEM, int CT>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSM)
-paged_decode_kernel(const __grid_constant__ PagedAttn a, const SchedShape shape) {
-    using C = DCfg<D, CT>;
-    extern __shared__ __align__(16) uint8_t smem[];
+template <int D, int ELEM, int CT, int NB>
+__global__ void __launch_bounds__(kThreads, DCfg<D, CT, NB>::PER_SM)
+paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
+                    const __grid_constant__ CUtensorMap tmV,
+                    const __grid_constant__ PagedAttn a, const SchedShape shape, const int box) {
+    using C = DCfg<D, CT, NB>;
+    constexpr int kRows = C::ROWS, kStages = C::STAGES;
+    constexpr float UNSCALE = Code<ELEM, CT>::kUnscale;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ uint64_t s_full[kWarps][kStages];
+    __shared__ int s_abort;
     __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
     __shared__ int s_last, s_bad[kRows];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
     const int block = blockIdx.x;
-    const uint32_t ring = smem_u32(smem) + warp * C::RING;
-    const float cscale = a.scale * kLog2e * (CT == kE4M3 ? Code<ELEM, CT>::kUnscale : 1.f);
+    uint8_t* ring = smem + warp * C::RING;
+    const uint32_t side = smem_u32(smem + C::SIDE_OFF) + warp * kStages * C::SIDE;
+    const float cscale = a.scale * kLog2e * UNSCALE;
+    if (threadIdx.x == 0) {
+        for (int w = 0; w < kWarps; w++)
+            for (int i = 0; i < kStages; i++) mbar_init(&s_full[w][i], 1);
+        s_abort = 0;
+        fence_mbar_init();
+    }
+    __syncthreads();
+    // where this lane's operands sit in a stage: K pieces t and t + 4 of row g,
+    // V piece g of rows 2t and 2t + 1 (swizzled as TMA stores them)
+    const uint32_t k_even = C::RB == 128 ? g * 128 + ((t ^ g) << 4) : g * 64 + ((t ^ (g >> 1)) << 4);
+    const uint32_t k_odd = k_even ^ 64;
+    const uint32_t v_even = C::RB == 128 ? 2 * t * 128 + ((g ^ (2 * t)) << 4)
+                                         : 2 * t * 64 + (((g >> 1) ^ t) << 4) + (g & 1) * 8;
+    const uint32_t v_odd = C::RB == 128 ? (2 * t + 1) * 128 + ((g ^ (2 * t + 1)) << 4) : v_even + 64;
+    // the boxes this lane fetches: K or V, box column, box row
+    const int box_kv = lane & 1, box_col = (lane >> 1) % C::CB, box_row = (lane >> 1) / C::CB;
+    const bool box_mine = box_row * box < C::BK;
+    uint32_t filled = 0, used = 0;                   // blocks so far
+    bool alive = true;
 
     Walker walk;
     walk.start(a, shape, block, gridDim.x);
     Segment sg;
     while (walk.next(a, shape, block, sg)) {
         const int rows = sg.ni * a.group;
-        const char* kbase = a.c.k + (long long)sg.head * a.c.head * C::EB;
-        const char* vbase = a.c.v + (long long)sg.head * a.c.head * C::EB;
         const float* ksb = a.c.ks + sg.head * a.c.shead;
         const float* vsb = a.c.vs + sg.head * a.c.shead;
         const int* table = a.table + sg.s * a.tstride;
-
-        // ---- queries: rows g and g + 8, dim permuted as the K pieces are
-        uint32_t qa[D / 16][4];
-        int lim[2];                                  // keys that the row sees
-#pragma unroll
-        for (int r = 0; r < 2; r++) {
-            const int row = g + 8 * r;
-            const bool live = row < rows;
-            const int tok = live ? row / a.group : 0;
-            const int hd = sg.head * a.group + (live ? row - tok * a.group : 0);
-            lim[r] = live ? tile_end(a, sg.q, sg.i0 + tok + 1) : 0;
-            const char* qrow = a.q + ((sg.q.q0 + sg.i0 + tok) * a.qr + hd * a.qh) * 2;
-            if constexpr (C::EB == 2) {
-#pragma unroll
-                for (int c = 0; c < D / 32; c++) {
-                    uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                    if (live) w = __ldg(reinterpret_cast<const uint4*>(qrow + c * 64 + t * 16));
-                    qa[2 * c][r] = w.x;
-                    qa[2 * c][r + 2] = w.y;
-                    qa[2 * c + 1][r] = w.z;
-                    qa[2 * c + 1][r + 2] = w.w;
-                }
-            } else {
-#pragma unroll
-                for (int c = 0; c < D / 64; c++)
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {    // 8 of the piece's 16 elements
-                        uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                        if (live)
-                            w = __ldg(reinterpret_cast<const uint4*>(qrow + c * 128 + t * 32 + h * 16));
-                        qa[4 * c + 2 * h][r] = w.x;
-                        qa[4 * c + 2 * h][r + 2] = w.y;
-                        qa[4 * c + 2 * h + 1][r] = w.z;
-                        qa[4 * c + 2 * h + 1][r + 2] = w.w;
-                    }
-            }
-        }
-        // below this key no row of the tile masks anything
-        const int lim_all = tile_end(a, sg.q, sg.i0 + 1);
-
-        float o[D / 8][4];
-#pragma unroll
-        for (int j = 0; j < D / 8; j++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) o[j][i] = 0.f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-        float vmost = 0.f, vpow = 1.f;               // fp16: see v_power
         const int stride = kWarps * C::BK;
         const int first = sg.k0 + warp * C::BK;
-        const int mine = sg.k1 > first ? (sg.k1 - first + stride - 1) / stride : 0;
+        const int mine = alive && sg.k1 > first ? (sg.k1 - first + stride - 1) / stride : 0;
 
         // ---- loads: block i into stage i % kStages
         constexpr int PL = C::BK > 32 ? 2 : 1;       // keys per lane
@@ -226,52 +210,51 @@ paged_decode_kernel(const __grid_constant__ PagedAttn a, const SchedShape shape)
             for (int h = 0; h < PL; h++) {
                 const int key = first + i * stride + h * 32 + lane;
                 page[h] = -2;                        // past the end
-                if (lane < C::BK && key < sg.k1) page[h] = __ldg(table + a.c.by_ps.div(key));
+                if ((C::BK >= 32 || lane < C::BK) && key < sg.k1)
+                    page[h] = __ldg(table + a.c.by_ps.div(key));
             }
         };
         auto load_block = [&](int i) {
-            const uint32_t st = ring + (i % kStages) * C::STAGE;
-            uint32_t at[PL];
+            const uint32_t stage = filled % kStages;
+            filled++;
             uint32_t there[PL];
 #pragma unroll
             for (int h = 0; h < PL; h++) {
-                const int key = first + i * stride + h * 32 + lane;
-                const int off = key - (int)a.c.by_ps.div(key) * a.c.ps;
-                const bool ok = page[h] >= 0 && page[h] < a.c.pages;
+                const bool ok = (unsigned)page[h] < (unsigned)a.c.pages;
                 if (!ok && page[h] != -2) note_bad_index();
-                at[h] = ok ? (uint32_t)((page[h] * a.c.page + off * a.c.row) * C::EB / 32) : kNone;
                 there[h] = __ballot_sync(0xffffffffu, ok);
                 if constexpr (C::Q8) {
-                    if (lane < C::BK) {
+                    if (C::BK >= 32 || lane < C::BK) {
+                        const int key = first + i * stride + h * 32 + lane;
+                        const int off = key - (int)a.c.by_ps.div(key) * a.c.ps;
                         const long long sat = ok ? page[h] * a.c.spage + off : 0;
-                        const uint32_t d = st + 8192 + (h * 32 + lane) * 4;
-                        copy_async<4>(d, reinterpret_cast<const char*>(ksb + sat), ok);
-                        copy_async<4>(d + C::BK * 4, reinterpret_cast<const char*>(vsb + sat), ok);
+                        const uint32_t d = side + stage * C::SIDE + 16 + (h * 32 + lane) * 4;
+                        copy_async4(d, ksb + sat, ok);
+                        copy_async4(d + C::BK * 4, vsb + sat, ok);
                     }
                 }
             }
             if (lane == 0) {
-                const uint32_t d = st + 8192 + (C::Q8 ? 2 * C::BK * 4 : 0);
-                asm volatile("st.shared.v2.u32 [%0], {%1,%2};"
-                             :: "r"(d), "r"(there[0]), "r"(there[PL - 1]) : "memory");
+                asm volatile("st.shared.v2.u32 [%0], {%1,%2};" :: "r"(side + stage * C::SIDE),
+                             "r"(there[0]), "r"(there[PL - 1]) : "memory");
+                mbar_expect_tx(&s_full[warp][stage], 8192);
             }
-#pragma unroll
-            for (int n = 0; n < C::NT; n++) {
-                const uint32_t x = __shfl_sync(0xffffffffu, at[PL > 1 ? n / 4 : 0], (n * 8 + g) & 31);
-                const char* p = kbase + (x == kNone ? 0ull : (unsigned long long)x * 32) + t * 16;
-#pragma unroll
-                for (int c = 0; c < C::KCH; c++)
-                    copy_async<16>(st + (n * C::KCH + c) * 512 + lane * 16, p + c * 64, x != kNone);
+            __syncwarp();
+            const int r = box_row * box;
+            int pg = __shfl_sync(0xffffffffu, page[0], r & 31);
+            if constexpr (PL > 1) {
+                const int p1 = __shfl_sync(0xffffffffu, page[1], r & 31);
+                if (r >= 32) pg = p1;
             }
-#pragma unroll
-            for (int n = 0; n < C::BK / 4; n++) {    // keys 2t, 2t+1, 2t+8, 2t+9 of each 16
-                const int key = (n >> 2) * 16 + 2 * t + (n & 1) + 8 * ((n >> 1) & 1);
-                const uint32_t x = __shfl_sync(0xffffffffu, at[PL > 1 ? n / 8 : 0], key & 31);
-                const char* p = vbase + (x == kNone ? 0ull : (unsigned long long)x * 32) + g * C::VP;
-#pragma unroll
-                for (int c = 0; c < C::VCH; c++)
-                    copy_async<C::VP>(st + 4096 + (n * C::VCH + c) * (32 * C::VP) + lane * C::VP,
-                                      p + c * 8 * C::VP, x != kNone);
+            if (box_mine) {
+                const int key = first + i * stride + r;
+                const int off = key - (int)a.c.by_ps.div(key) * a.c.ps;
+                // a page that is not there, or not wanted, is asked for out of
+                // range and arrives as zeros
+                if ((unsigned)pg >= (unsigned)a.c.pages) pg = a.c.pages;
+                tma_load_4d(ring + stage * 8192 + box_kv * 4096 + box_col * (C::BK * C::RB) + r * C::RB,
+                            box_kv ? &tmV : &tmK, &s_full[warp][stage], box_col * (128 / C::EB), off,
+                            sg.head, pg);
             }
         };
 
@@ -282,148 +265,226 @@ paged_decode_kernel(const __grid_constant__ PagedAttn a, const SchedShape shape)
             fetch_pages(i + 1);
             copy_commit();
         }
+
+        // ---- queries: row nb * 8 + g, dim permuted as the K pieces are
+        uint32_t qb[D / 16][NB][2];
+        int lim[NB][2];                              // keys that rows nb*8 + 2t, + 1 see
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) {
+            const int row = nb * 8 + g;
+            const bool live = row < rows;
+            const RowPlace pl = row_place(a, sg, live ? row : 0);
+            const char* qrow = a.q + (pl.token * a.qr + pl.head * a.qh) * 2;
+            // 16-byte pieces of q: one for two 16-bit steps, half of one K piece of codes
+#pragma unroll
+            for (int c = 0; c < D / 32; c++) {
+                const int at = C::EB == 2 ? c * 64 + t * 16 : (c >> 1) * 128 + t * 32 + (c & 1) * 16;
+                uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                if (live) w = __ldg(reinterpret_cast<const uint4*>(qrow + at));
+                qb[2 * c][nb][0] = w.x;
+                qb[2 * c][nb][1] = w.y;
+                qb[2 * c + 1][nb][0] = w.z;
+                qb[2 * c + 1][nb][1] = w.w;
+            }
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int r = nb * 8 + 2 * t + e;
+                lim[nb][e] = r < rows ? tile_end(a, sg.q, sg.i0 + r / a.group + 1) : 0;
+            }
+        }
+        // up to this key no row of the tile masks anything
+        const int lim_all = tile_end(a, sg.q, sg.i0 + 1);
+
+        float o[D / 16][NB][4];
+        float m[NB][2], base[NB][2], l[NB][2];
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) {
+#pragma unroll
+            for (int j = 0; j < D / 16; j++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[j][nb][i] = 0.f;
+            m[nb][0] = m[nb][1] = -INFINITY;
+            base[nb][0] = base[nb][1] = 0.f;
+            l[nb][0] = l[nb][1] = 0.f;
+        }
+        float vmost = 0.f, vpow = 1.f, lpow = 0.f;   // fp16: see v_power
+
         for (int i = 0; i < mine; i++) {
-            copy_wait<kStages - 2>();
-            __syncwarp();
+            __syncwarp();                            // the stage to fill is no longer read
             if (i + kStages - 1 < mine) load_block(i + kStages - 1);
             fetch_pages(i + kStages);
             copy_commit();
-            const uint32_t st = ring + (i % kStages) * C::STAGE;
+            const uint32_t stage = used % kStages;
+            const uint32_t st = smem_u32(ring) + stage * 8192, sc = side + stage * C::SIDE;
+            copy_wait<kStages - 1>();
+            alive = __all_sync(0xffffffffu, mbar_wait(&s_full[warp][stage], (used / kStages) & 1, &s_abort));
+            if (!alive) break;
+            used++;
             const int kb = first + i * stride;
+            // V rows past the keys, in a box that is partly wanted, may hold
+            // anything: 0 times them must be 0
+            const int left = sg.k1 - kb;
+            if (left < C::BK) {
+                constexpr int PIECES = C::RB / 16;
+                for (int j = lane; j < (C::BK - left) * PIECES * C::CB; j += 32) {
+                    const int row = left + j / (PIECES * C::CB), c = j % (PIECES * C::CB);
+                    *reinterpret_cast<uint4*>(ring + stage * 8192 + 4096 + (c / PIECES) * (C::BK * C::RB) +
+                                              row * C::RB + (c % PIECES) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                }
+                fence_async_smem();                  // before TMA fills the stage again
+                __syncwarp();
+            }
 
-            // ---- scores
-            float x[C::NT][4];
+            // ---- scores: keys g and g + 8 of each 16, rows 2t and 2t + 1
+            float x[C::BK / 16][NB][4];
 #pragma unroll
-            for (int n = 0; n < C::NT; n++) {
-                x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.f;
+            for (int kk = 0; kk < C::BK / 16; kk++) {
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++)
+                    x[kk][nb][0] = x[kk][nb][1] = x[kk][nb][2] = x[kk][nb][3] = 0.f;
 #pragma unroll
                 for (int c = 0; c < C::KCH; c++) {
-                    const uint4 w = lds16(st + (n * C::KCH + c) * 512 + lane * 16);
+                    const uint32_t p = st + (c & 1 ? k_odd : k_even) + (c >> 1) * (C::BK * C::RB) +
+                                       kk * 16 * C::RB;
+                    const uint4 w = lds16(p), v = lds16(p + 8 * C::RB);
                     if constexpr (C::EB == 2) {
-                        mma16<ELEM>(x[n], qa[2 * c], w.x, w.y);
-                        mma16<ELEM>(x[n], qa[2 * c + 1], w.z, w.w);
+#pragma unroll
+                        for (int nb = 0; nb < NB; nb++) {
+                            mma16<ELEM>(x[kk][nb], w.x, v.x, w.y, v.y, qb[2 * c][nb]);
+                            mma16<ELEM>(x[kk][nb], w.z, v.z, w.w, v.w, qb[2 * c + 1][nb]);
+                        }
                     } else {
-                        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+                        const uint32_t wu[4] = {w.x, w.y, w.z, w.w}, vu[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            uint32_t b0, b1;
-                            Code<ELEM, CT>::widen(u[e], b0, b1);
-                            mma16<ELEM>(x[n], qa[4 * c + e], b0, b1);
+                            uint32_t a0, a1, a2, a3;
+                            Code<ELEM, CT>::widen(wu[e], a0, a2);
+                            Code<ELEM, CT>::widen(vu[e], a1, a3);
+#pragma unroll
+                            for (int nb = 0; nb < NB; nb++)
+                                mma16<ELEM>(x[kk][nb], a0, a1, a2, a3, qb[4 * c + e][nb]);
                         }
                     }
                 }
             }
-            const uint2 there = lds8(st + 8192 + (C::Q8 ? 2 * C::BK * 4 : 0));
-            const uint32_t all = C::BK >= 32 ? 0xffffffffu : (1u << C::BK) - 1u;
-            const bool edge = kb + C::BK > lim_all || there.x != all || there.y != all;
+            const uint2 there = lds8(sc);
+            constexpr uint32_t ALL = C::BK >= 32 ? 0xffffffffu : (1u << (C::BK & 31)) - 1u;
+            const bool edge = kb + C::BK > lim_all || there.x != ALL || there.y != ALL;
+            bool grow = false;
+            float alpha[NB][2];
 #pragma unroll
-            for (int n = 0; n < C::NT; n++) {
+            for (int kk = 0; kk < C::BK / 16; kk++) {
                 float f0 = cscale, f1 = cscale;
                 if constexpr (C::Q8) {
-                    const uint2 ks = lds8(st + 8192 + (n * 8 + 2 * t) * 4);
-                    f0 *= __uint_as_float(ks.x);
-                    f1 *= __uint_as_float(ks.y);
+                    f0 *= __uint_as_float(lds4(sc + 16 + (kk * 16 + g) * 4));
+                    f1 *= __uint_as_float(lds4(sc + 16 + (kk * 16 + g + 8) * 4));
                 }
-                x[n][0] *= f0;
-                x[n][1] *= f1;
-                x[n][2] *= f0;
-                x[n][3] *= f1;
-                if (edge) {
-                    const uint32_t mask = PL > 1 && n >= 4 ? there.y : there.x;
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const int j = n * 8 + 2 * t + e;
+                for (int nb = 0; nb < NB; nb++) {
+                    x[kk][nb][0] *= f0;
+                    x[kk][nb][1] *= f0;
+                    x[kk][nb][2] *= f1;
+                    x[kk][nb][3] *= f1;
+                }
+                if (edge) {
+                    const uint32_t mask = PL > 1 && kk >= 2 ? there.y : there.x;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const int j = kk * 16 + g + 8 * h;
                         const bool here = (mask >> (j & 31)) & 1u;
-                        if (!here || kb + j >= lim[0]) x[n][e] = -INFINITY;
-                        if (!here || kb + j >= lim[1]) x[n][2 + e] = -INFINITY;
+#pragma unroll
+                        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                            for (int e = 0; e < 2; e++)
+                                if (!here || kb + j >= lim[nb][e]) x[kk][nb][2 * h + e] = -INFINITY;
                     }
                 }
             }
 
             // ---- running maximum
-            float alpha[2] = {1.f, 1.f}, base[2];
-            bool grow = false;
 #pragma unroll
-            for (int r = 0; r < 2; r++) {
-                float mx = x[0][2 * r];
+            for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-                for (int n = 0; n < C::NT; n++) mx = fmaxf(mx, fmaxf(x[n][2 * r], x[n][2 * r + 1]));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                if (mx > m[r] + kLazy) {             // also from -inf
-                    alpha[r] = ex2(m[r] - mx);
-                    m[r] = mx;
-                    grow = true;
+                for (int e = 0; e < 2; e++) {
+                    float mx = fmaxf(x[0][nb][e], x[0][nb][2 + e]);
+#pragma unroll
+                    for (int kk = 1; kk < C::BK / 16; kk++)
+                        mx = fmaxf(mx, fmaxf(x[kk][nb][e], x[kk][nb][2 + e]));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                    alpha[nb][e] = 1.f;
+                    if (mx > m[nb][e] + kLazy) {     // also from -inf
+                        alpha[nb][e] = ex2(m[nb][e] - mx);
+                        m[nb][e] = mx;
+                        grow = true;
+                    }
                 }
-                base[r] = m[r] == -INFINITY ? 0.f : m[r];
-            }
             float vfix = 1.f;
             if constexpr (C::Q8 && ELEM == kF16) {
                 float big = 0.f;
-                if (lane < C::BK) {
-                    big = __uint_as_float(lds4(st + 8192 + (C::BK + lane) * 4));
-                    if (PL > 1)
-                        big = fmaxf(big, __uint_as_float(lds4(st + 8192 + (C::BK + 32 + lane) * 4)));
-                }
+                if (C::BK >= 32 || lane < C::BK)
+                    big = __uint_as_float(lds4(sc + 16 + (C::BK + lane) * 4));
+                if (PL > 1)
+                    big = fmaxf(big, __uint_as_float(lds4(sc + 16 + (C::BK + 32 + lane) * 4)));
 #pragma unroll
                 for (int o2 = 16; o2 > 0; o2 >>= 1)
                     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o2));
                 vfix = v_power(big, vmost, vpow);
+                if (vfix != 1.f) lpow = log2f(vpow); // a power of two: exact
                 grow = grow || vfix != 1.f;
             }
             if (__any_sync(0xffffffffu, grow)) {
-                l[0] *= alpha[0];
-                l[1] *= alpha[1];
 #pragma unroll
-                for (int j = 0; j < D / 8; j++) {
-                    o[j][0] *= alpha[0] * vfix;
-                    o[j][1] *= alpha[0] * vfix;
-                    o[j][2] *= alpha[1] * vfix;
-                    o[j][3] *= alpha[1] * vfix;
-                }
+                for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const float f = alpha[nb][e] * vfix;
+                        // the power of two rides in the exponent, on O and l alike
+                        base[nb][e] = (m[nb][e] == -INFINITY ? 0.f : m[nb][e]) - lpow;
+                        l[nb][e] *= f;
+#pragma unroll
+                        for (int j = 0; j < D / 16; j++) {
+                            o[j][nb][e] *= f;
+                            o[j][nb][2 + e] *= f;
+                        }
+                    }
             }
 
             // ---- weights, and P.V sixteen keys at a time
 #pragma unroll
             for (int kk = 0; kk < C::BK / 16; kk++) {
-                uint32_t pa[4];
+                float v0 = 1.f, v1 = 1.f;
+                if constexpr (C::Q8) {
+                    v0 = __uint_as_float(lds4(sc + 16 + (C::BK + kk * 16 + g) * 4));
+                    v1 = __uint_as_float(lds4(sc + 16 + (C::BK + kk * 16 + g + 8) * 4));
+                }
+                uint32_t pb[NB][2];
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int n = 2 * kk + h;
+                for (int nb = 0; nb < NB; nb++) {
                     float p[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        p[e] = ex2(x[n][e] - base[e >> 1]);
-                        l[e >> 1] += p[e];
+                        p[e] = ex2(x[kk][nb][e] - base[nb][e & 1]);
+                        l[nb][e & 1] += p[e];
                     }
                     if constexpr (C::Q8) {
-                        const uint2 vs = lds8(st + 8192 + (C::BK + n * 8 + 2 * t) * 4);
-                        float v0 = __uint_as_float(vs.x), v1 = __uint_as_float(vs.y);
-                        if constexpr (ELEM == kF16) {
-                            v0 *= vpow;
-                            v1 *= vpow;
-                        }
+                        // (a masked key's scale may be NaN: paged_finish.cuh)
                         p[0] *= v0;
-                        p[1] *= v1;
-                        p[2] *= v0;
+                        p[1] *= v0;
+                        p[2] *= v1;
                         p[3] *= v1;
-                        if (edge) {                  // 0 * NaN: a masked key's scale
-                            if (x[n][0] == -INFINITY) p[0] = 0.f;
-                            if (x[n][1] == -INFINITY) p[1] = 0.f;
-                            if (x[n][2] == -INFINITY) p[2] = 0.f;
-                            if (x[n][3] == -INFINITY) p[3] = 0.f;
-                        }
                     }
-                    pa[2 * h] = pack2<ELEM>(p[0], p[1]);
-                    pa[2 * h + 1] = pack2<ELEM>(p[2], p[3]);
+                    pb[nb][0] = transpose8(pack2<ELEM>(p[0], p[1]));
+                    pb[nb][1] = transpose8(pack2<ELEM>(p[2], p[3]));
                 }
 #pragma unroll
                 for (int c = 0; c < C::VCH; c++) {
                     uint32_t w[4][C::VP / 4];
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        const uint32_t p = st + 4096 + ((kk * 4 + k) * C::VCH + c) * (32 * C::VP) +
-                                           lane * C::VP;
+                        const uint32_t p = st + 4096 + (k & 1 ? v_odd : v_even) + c * (C::BK * C::RB) +
+                                           (kk * 16 + (k >> 1) * 8) * C::RB;
                         if constexpr (C::VP == 16) {
                             const uint4 v = lds16(p);
                             w[k][0] = v.x; w[k][1] = v.y; w[k][2] = v.z; w[k][3] = v.w;
@@ -432,23 +493,27 @@ paged_decode_kernel(const __grid_constant__ PagedAttn a, const SchedShape shape)
                             w[k][0] = v.x; w[k][1] = v.y;
                         }
                     }
+                    // columns e and e + 1 of this lane's VE: output rows g, g + 8
 #pragma unroll
                     for (int i4 = 0; i4 < C::VP / 4; i4++) {
                         if constexpr (C::EB == 2) {
-                            mma16<ELEM>(o[c * C::VE + 2 * i4], pa, prmt(w[0][i4], w[1][i4], 0x5410),
-                                        prmt(w[2][i4], w[3][i4], 0x5410));
-                            mma16<ELEM>(o[c * C::VE + 2 * i4 + 1], pa,
-                                        prmt(w[0][i4], w[1][i4], 0x7632),
-                                        prmt(w[2][i4], w[3][i4], 0x7632));
+                            const uint32_t a0 = prmt(w[0][i4], w[1][i4], 0x5410);
+                            const uint32_t a1 = prmt(w[0][i4], w[1][i4], 0x7632);
+                            const uint32_t a2 = prmt(w[2][i4], w[3][i4], 0x5410);
+                            const uint32_t a3 = prmt(w[2][i4], w[3][i4], 0x7632);
+#pragma unroll
+                            for (int nb = 0; nb < NB; nb++)
+                                mma16<ELEM>(o[c * C::VE / 2 + i4][nb], a0, a1, a2, a3, pb[nb]);
                         } else {
 #pragma unroll
                             for (int h = 0; h < 2; h++) {
                                 const uint32_t sel = h ? 0x7362 : 0x5140;
-                                uint32_t lo0, hi0, lo1, hi1;
-                                Code<ELEM, CT>::widen(prmt(w[0][i4], w[1][i4], sel), lo0, hi0);
-                                Code<ELEM, CT>::widen(prmt(w[2][i4], w[3][i4], sel), lo1, hi1);
-                                mma16<ELEM>(o[c * C::VE + 4 * i4 + 2 * h], pa, lo0, lo1);
-                                mma16<ELEM>(o[c * C::VE + 4 * i4 + 2 * h + 1], pa, hi0, hi1);
+                                uint32_t a0, a1, a2, a3;
+                                Code<ELEM, CT>::widen(prmt(w[0][i4], w[1][i4], sel), a0, a1);
+                                Code<ELEM, CT>::widen(prmt(w[2][i4], w[3][i4], sel), a2, a3);
+#pragma unroll
+                                for (int nb = 0; nb < NB; nb++)
+                                    mma16<ELEM>(o[c * C::VE / 2 + 2 * i4 + h][nb], a0, a1, a2, a3, pb[nb]);
                             }
                         }
                     }
@@ -459,28 +524,32 @@ paged_decode_kernel(const __grid_constant__ PagedAttn a, const SchedShape shape)
 
         // ---- join the warps: maxima and sums, then O through shared memory
 #pragma unroll
-        for (int r = 0; r < 2; r++) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-            if (t == 0) {
-                s_m[warp][g + 8 * r] = m[r];
-                s_l[warp][g + 8 * r] = l[r];
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                float sum = l[nb][e];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                if (g == 0) {
+                    s_m[warp][nb * 8 + 2 * t + e] = m[nb][e] - lpow;
+                    s_l[warp][nb * 8 + 2 * t + e] = sum;
+                }
             }
-        }
+        if (threadIdx.x < kRows) s_bad[threadIdx.x] = 0;
         __syncthreads();                             // also: every ring is drained
         float* so = reinterpret_cast<float*>(smem);  // [warp][row][D + 4]
-        const float unv = (CT == kE4M3 ? Code<ELEM, CT>::kUnscale : 1.f) / vpow;
 #pragma unroll
-        for (int c = 0; c < C::VCH; c++)
+        for (int j = 0; j < D / 16; j++)
 #pragma unroll
-            for (int e = 0; e < C::VE; e++)
+            for (int nb = 0; nb < NB; nb++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const int row = g + 8 * (i >> 1);
-                    const int d = c * 8 * C::VE + (2 * t + (i & 1)) * C::VE + e;
-                    if (row < rows) so[(warp * kRows + row) * (D + 4) + d] = o[c * C::VE + e][i] * unv;
+                    const int row = nb * 8 + 2 * t + (i & 1);
+                    const int e = 2 * j + (i >> 1);  // column within the lane's pieces
+                    const int d = (e / C::VE) * 8 * C::VE + g * C::VE + e % C::VE;
+                    if (row < rows) so[(warp * kRows + row) * (D + 4) + d] = o[j][nb][i] * UNSCALE;
                 }
-        if (threadIdx.x < kRows) s_bad[threadIdx.x] = 0;
         __syncthreads();
         const bool whole = sg.parts == 1;
         float* slot = whole ? nullptr : part_slot(a, kRows, block, sg.part == 0);
@@ -536,14 +605,55 @@ paged_decode_kernel(const __grid_constant__ PagedAttn a, const SchedShape shape)
         }
         __syncthreads();
         if (final) repair_rows(a, sg, rows, s_bad, warp, kWarps);
+        fence_async_smem();                          // the rings are TMA's again
         __syncthreads();
     }
 }
 
-template <int D, int ELEM, int CT>
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                              const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+    static std::atomic<EncodeFn> fn{nullptr};
+    EncodeFn f = fn.load();
+    if (f) return f;
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) ==
+            cudaSuccess && q == cudaDriverEntryPointSuccess) {
+        f = reinterpret_cast<EncodeFn>(ptr);
+        fn.store(f);
+    }
+    return f;
+}
+
+// {dim, page_size, heads, pages}, boxes of `box` rows of row_bytes
+bool cache_map(CUtensorMap* tm, const PagedAttn& a, const void* base, int row_bytes, int box_rows) {
+    EncodeFn enc = encode_fn();
+    if (!enc) return false;
+    const int eb = a.type >= kI8 ? 1 : 2;
+    const cuuint64_t dims[4] = {(cuuint64_t)a.c.dim, (cuuint64_t)a.c.ps, (cuuint64_t)a.c.heads,
+                                (cuuint64_t)a.c.pages};
+    const cuuint64_t st[3] = {a.c.ps > 1 ? (cuuint64_t)a.c.row * eb : 16,
+                              a.c.heads > 1 ? (cuuint64_t)a.c.head * eb : 16,
+                              a.c.pages > 1 ? (cuuint64_t)a.c.page * eb : 16};
+    const cuuint32_t box[4] = {(cuuint32_t)(row_bytes / eb), (cuuint32_t)box_rows, 1, 1};
+    const cuuint32_t ones[4] = {1, 1, 1, 1};
+    const CUtensorMapDataType type = a.type >= kI8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : a.type == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                     : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    return enc(tm, type, 4, const_cast<void*>(base), dims, st, box, ones,
+               CU_TENSOR_MAP_INTERLEAVE_NONE,
+               row_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, int ELEM, int CT, int NB>
 int launch(const PagedAttn& a, cudaStream_t s) {
-    using C = DCfg<D, CT>;
-    auto kern = paged_decode_kernel<D, ELEM, CT>;
+    using C = DCfg<D, CT, NB>;
+    auto kern = paged_decode_kernel<D, ELEM, CT, NB>;
     static std::atomic<unsigned long long> attr_set{0};
     int dev = 0;
     cudaGetDevice(&dev);
@@ -554,24 +664,45 @@ int launch(const PagedAttn& a, cudaStream_t s) {
         if (e != cudaSuccess) return (int)e;
         attr_set.fetch_or(bit);
     }
-    const SchedShape shape{kRows / a.group, kWarps * C::BK, 2};
-    kern<<<decode_blocks(), kThreads, C::SMEM, s>>>(a, shape);
+    const SchedShape shape{C::ROWS / a.group, kWarps * C::BK, 2};
+    int box = 8;                                     // tokens of a page side by side
+    while (box < C::BK && a.c.ps % (2 * box) == 0) box *= 2;
+    CUtensorMap tk, tv;
+    if (!cache_map(&tk, a, a.c.k, C::RB, box) || !cache_map(&tv, a, a.c.v, C::RB, box)) return 1;
+    kern<<<std::min(C::PER_SM * num_sms(), kMaxBlocks), kThreads, C::SMEM, s>>>(tk, tv, a, shape, box);
     const cudaError_t e = cudaGetLastError();
     if (e == cudaSuccess) note_launch();
     return e == cudaSuccess ? 0 : (int)e;
 }
 
+// row blocks of 8: those of the longest chunk, as the caller tells it
+int row_blocks(const PagedAttn& a) {
+    const long long rows = (long long)std::max(1, a.max_q) * a.group;
+    return (int)std::min<long long>((rows + 7) / 8, kMaxNB);
+}
+
+template <int D, int ELEM, int CT>
+int launch_rows(const PagedAttn& a, cudaStream_t s) {
+    switch (row_blocks(a)) {
+    case 1: return launch<D, ELEM, CT, 1>(a, s);
+    case 2: return launch<D, ELEM, CT, 2>(a, s);
+    default: return launch<D, ELEM, CT, 3>(a, s);
+    }
+}
+
 template <int ELEM, int CT>
 int launch_dim(const PagedAttn& a, cudaStream_t s) {
-    return a.c.dim == 128 ? launch<128, ELEM, CT>(a, s) : launch<64, ELEM, CT>(a, s);
+    return a.c.dim == 128 ? launch_rows<128, ELEM, CT>(a, s) : launch_rows<64, ELEM, CT>(a, s);
 }
 
 }  // namespace
 
-int decode_blocks() { return std::min(kBlocksPerSM * num_sms(), kMaxBlocks); }
+int decode_max_rows() { return 8 * kMaxNB; }
 
 size_t paged_decode_workspace(const PagedAttn& a) {
-    return kCounterBytes + 2ull * decode_blocks() * slot_floats(kRows, a.c.dim) * sizeof(float);
+    const int nb = row_blocks(a), per_sm = nb == 1 ? 3 : 2;
+    const int blocks = std::min(per_sm * num_sms(), kMaxBlocks);
+    return kCounterBytes + 2ull * blocks * slot_floats(8 * nb, a.c.dim) * sizeof(float);
 }
 
 int paged_decode(const PagedAttn& a, cudaStream_t s) {
