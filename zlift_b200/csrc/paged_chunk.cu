@@ -160,7 +160,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
     constexpr int NSLOT = C::NSLOT, KV_BARS = C::KV_BARS;
     constexpr uint32_t IDESC_QK = make_idesc(1, ELEM == kBF16 ? 1 : 0, 0, 0, BQ, BKEY);
     constexpr uint32_t IDESC_PV = make_idesc(1, ELEM == kBF16 ? 1 : 0, 0, 1, BQ, D);
-    constexpr float UNSCALE = Code<ELEM, CT>::kUnscale;
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -191,7 +190,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
     }
     {
         Walker w;
-        w.start(a, shape.sched, blockIdx.x, gridDim.x);
+        w.start(a, shape.sched, blockIdx.x);
         if (lane == 0) sd.walk[warp] = w;
     }
     tc_fence_before();
@@ -471,7 +470,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
         const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
         const uint32_t s_addr = tmem_base + lane_off + (t ? C::S_COL1 : C::S_COL0);
         const uint32_t o_addr = tmem_base + lane_off + (t ? C::O_COL1 : C::O_COL0);
-        const float c = a.scale * kLog2e * UNSCALE;
+        const float c = a.scale * kLog2e;
         // weights reach 2^lazy; in fp16 times a V scale of up to 512
         constexpr float kLazyLog2 = Q8 && ELEM == kF16 ? 6.f : 8.f;
         uint32_t step = 0, tiles = 0, finals = 0;
@@ -616,10 +615,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
 #pragma unroll
                         for (int i = 0; i < 8; i++)
                             *reinterpret_cast<float4*>(ps + 2 * BQ + ((c0 / 4 + i) * BQ + r) * 4) =
-                                make_float4(__uint_as_float(v[4 * i]) * UNSCALE,
-                                            __uint_as_float(v[4 * i + 1]) * UNSCALE,
-                                            __uint_as_float(v[4 * i + 2]) * UNSCALE,
-                                            __uint_as_float(v[4 * i + 3]) * UNSCALE);
+                                make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]),
+                                            __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
                     }
                 }
                 __threadfence();
@@ -647,7 +644,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                 }
             }
             if (final && alive) {
-                const float inv = l == 0.f ? 0.f : (split ? 1.f : UNSCALE) / l;
+                const float inv = l == 0.f ? 0.f : 1.f / l;
                 const RowPlace pl = row_place(a, sg, row_ok ? r : 0);
                 char* orow = a.o + (pl.token * a.orow + pl.head * a.oh) * 2;
                 float z = 0.f;
@@ -751,7 +748,7 @@ int launch(const PagedAttn& a, cudaStream_t s) {
     using C = PCfg<D, (CT >= kI8)>;
     ChunkShape shape;
     shape.tile_tokens = BQ / a.group;
-    shape.sched = SchedShape{2 * shape.tile_tokens, BKEY, 2};
+    shape.sched = SchedShape{2 * shape.tile_tokens, BKEY, 2, chunk_blocks(), 0, 256};
     shape.box = 8;
     while (shape.box < BKEY && a.c.ps % (2 * shape.box) == 0) shape.box *= 2;
     CUtensorMap tq, tk, tv;

@@ -5,16 +5,13 @@
 namespace zl {
 
 // widen(u, lo, hi): the four codes in u as two pairs of 16-bit values (codes 0
-// and 1 in lo, 2 and 3 in hi), each the code's value divided by kUnscale.
+// and 1 in lo, 2 and 3 in hi)
 template <int ELEM, int CT>
-struct Code {                            // a 16-bit cache: nothing to widen
-    static constexpr float kUnscale = 1.f;
-};
+struct Code {};                          // a 16-bit cache: nothing to widen
 
 // int8 -> fp16: 0x6400 | (c + 128) is 1024 + 128 + c
 template <>
 struct Code<kF16, kI8> {
-    static constexpr float kUnscale = 1.f;
     static __device__ __forceinline__ void widen(uint32_t u, uint32_t& lo, uint32_t& hi) {
         const uint32_t x = u ^ 0x80808080u;
         const uint32_t k = 0x64806480u;              // 1152
@@ -31,7 +28,6 @@ struct Code<kF16, kI8> {
 // with c = low7 - 128 * sign, (128 + low7) - (128 or 256, by the sign) = c
 template <>
 struct Code<kBF16, kI8> {
-    static constexpr float kUnscale = 1.f;
     static __device__ __forceinline__ uint32_t half(uint32_t y) {   // bytes c, 0x43, c, 0x43
         uint32_t a = y & 0xff7fff7fu, b = y & 0xff80ff80u;
         const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a),
@@ -44,27 +40,22 @@ struct Code<kBF16, kI8> {
     }
 };
 
-// e4m3 -> fp16: sign, 4 exponent and 3 mantissa bits moved into place; the
-// exponent bias differs by 8, so the value is 2^-8 of the code's, subnormal
-// codes included (fp16's own subnormals hold them).  The caller multiplies
-// the product by kUnscale.
+// e4m3 -> fp16 by the hardware's conversion of two codes (exact)
 template <>
 struct Code<kF16, kE4M3> {
-    static constexpr float kUnscale = 256.f;
-    static __device__ __forceinline__ uint32_t half(uint32_t p) {   // codes in the high bytes
-        return (p & 0x80008000u) | ((p >> 1) & 0x3f803f80u);
-    }
     static __device__ __forceinline__ void widen(uint32_t u, uint32_t& lo, uint32_t& hi) {
-        lo = half(__byte_perm(u, 0u, 0x1404));
-        hi = half(__byte_perm(u, 0u, 0x3424));
+        const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(u & 0xffffu), __NV_E4M3);
+        const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(u >> 16), __NV_E4M3);
+        lo = (uint32_t)a.x | (uint32_t)a.y << 16;
+        hi = (uint32_t)b.x | (uint32_t)b.y << 16;
     }
 };
 
-// e4m3 -> bf16: the same, 2^-120 of the code's value; brought back at once,
-// for products that small would leave fp32's normal range
+// e4m3 -> bf16: sign, 4 exponent and 3 mantissa bits moved into place, which
+// is 2^-120 of the code's value (the exponent biases differ by 120; subnormal
+// codes become bf16 subnormals), brought back by an exact product
 template <>
 struct Code<kBF16, kE4M3> {
-    static constexpr float kUnscale = 1.f;
     static __device__ __forceinline__ uint32_t half(uint32_t p) {
         uint32_t x = (p & 0x80008000u) | ((p >> 4) & 0x07f007f0u);
         const uint32_t k = 0x7b807b80u;              // 2^120

@@ -48,6 +48,9 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMaxNB = 3;
+constexpr int kLeast = 2;                // steps of a piece, at least
+constexpr int kExtra = 2;                // small pieces for each large one
+constexpr int kShare = 200;              // 256ths of the work in large pieces
 constexpr float kLazy = 6.f;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -132,6 +135,33 @@ __device__ __forceinline__ void copy_wait() {
     asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory");
 }
 
+// N (2 or 4) floats at an address aligned for them
+template <int N>
+__device__ __forceinline__ void load_vec(float (&x)[N], const float* p) {
+    if constexpr (N == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(p);
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    } else {
+        const float2 v = *reinterpret_cast<const float2*>(p);
+        x[0] = v.x; x[1] = v.y;
+    }
+}
+template <int N>
+__device__ __forceinline__ void load_vec_cg(float (&x)[N], const float* p) {
+    if constexpr (N == 4) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(p));
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    } else {
+        const float2 v = __ldcg(reinterpret_cast<const float2*>(p));
+        x[0] = v.x; x[1] = v.y;
+    }
+}
+template <int N>
+__device__ __forceinline__ void store_vec(float* p, const float (&x)[N]) {
+    if constexpr (N == 4) *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    else *reinterpret_cast<float2*>(p) = make_float2(x[0], x[1]);
+}
+
 __device__ __forceinline__ uint4 lds16(uint32_t a) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
@@ -149,6 +179,32 @@ __device__ __forceinline__ uint32_t lds4(uint32_t a) {
     return v;
 }
 
+// Row block nb of the query operand from bf16 to fp16, the type that codes
+// widen to most cheaply and weights keep most bits in.  A row is brought to a
+// maximum of [1, 2) by a power of two (returned: its inverse): bf16's 8 bits fit
+// fp16's 11, and what lies 2^14 below the row's maximum and loses bits to
+// fp16's subnormals is off by 2^-25 of that maximum, as fp32 sums are.
+template <int D, int NB>
+__device__ __forceinline__ float halve_row(uint32_t (&qb)[D / 16][NB][2], int nb) {
+    unsigned most = 0;
+#pragma unroll
+    for (int i = 0; i < D / 16; i++)
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+            most = max(most, max(qb[i][nb][h] << 16 & 0x7fffffffu, qb[i][nb][h] & 0x7fff0000u));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    const int e = most ? min(max((int)(most >> 23) - 127, -120), 120) : 0;
+    const float f = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+    for (int i = 0; i < D / 16; i++)
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+            qb[i][nb][h] = pack2<kF16>(__uint_as_float(qb[i][nb][h] << 16) * f,
+                                       __uint_as_float(qb[i][nb][h] & 0xffff0000u) * f);
+    return __uint_as_float((uint32_t)(127 + e) << 23);
+}
+
 template <int D, int ELEM, int CT, int NB>
 __global__ void __launch_bounds__(kThreads, DCfg<D, CT, NB>::PER_SM)
 paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
@@ -156,7 +212,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
                     const __grid_constant__ PagedAttn a, const SchedShape shape, const int box) {
     using C = DCfg<D, CT, NB>;
     constexpr int kRows = C::ROWS, kStages = C::STAGES;
-    constexpr float UNSCALE = Code<ELEM, CT>::kUnscale;
+    constexpr int MT = C::Q8 ? kF16 : ELEM;          // type of the products' operands
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -169,7 +225,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
     const int block = blockIdx.x;
     uint8_t* ring = smem + warp * C::RING;
     const uint32_t side = smem_u32(smem + C::SIDE_OFF) + warp * kStages * C::SIDE;
-    const float cscale = a.scale * kLog2e * UNSCALE;
+    const float cscale = a.scale * kLog2e;
     if (threadIdx.x == 0) {
         for (int w = 0; w < kWarps; w++)
             for (int i = 0; i < kStages; i++) mbar_init(&s_full[w][i], 1);
@@ -191,7 +247,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
     bool alive = true;
 
     Walker walk;
-    walk.start(a, shape, block, gridDim.x);
+    walk.start(a, shape, block);
     Segment sg;
     while (walk.next(a, shape, block, sg)) {
         const int rows = sg.ni * a.group;
@@ -268,6 +324,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
 
         // ---- queries: row nb * 8 + g, dim permuted as the K pieces are
         uint32_t qb[D / 16][NB][2];
+        float qscale[NB][2];                         // of rows nb*8 + 2t, + 1 (8-bit caches)
         int lim[NB][2];                              // keys that rows nb*8 + 2t, + 1 see
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) {
@@ -285,6 +342,13 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
                 qb[2 * c][nb][1] = w.y;
                 qb[2 * c + 1][nb][0] = w.z;
                 qb[2 * c + 1][nb][1] = w.w;
+            }
+            if constexpr (C::Q8 && ELEM == kBF16) {
+                const float f = halve_row<D>(qb, nb);
+                qscale[nb][0] = cscale * __shfl_sync(0xffffffffu, f, 8 * t);
+                qscale[nb][1] = cscale * __shfl_sync(0xffffffffu, f, 8 * t + 4);
+            } else {
+                qscale[nb][0] = qscale[nb][1] = cscale;
             }
 #pragma unroll
             for (int e = 0; e < 2; e++) {
@@ -350,19 +414,19 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
                     if constexpr (C::EB == 2) {
 #pragma unroll
                         for (int nb = 0; nb < NB; nb++) {
-                            mma16<ELEM>(x[kk][nb], w.x, v.x, w.y, v.y, qb[2 * c][nb]);
-                            mma16<ELEM>(x[kk][nb], w.z, v.z, w.w, v.w, qb[2 * c + 1][nb]);
+                            mma16<MT>(x[kk][nb], w.x, v.x, w.y, v.y, qb[2 * c][nb]);
+                            mma16<MT>(x[kk][nb], w.z, v.z, w.w, v.w, qb[2 * c + 1][nb]);
                         }
                     } else {
                         const uint32_t wu[4] = {w.x, w.y, w.z, w.w}, vu[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             uint32_t a0, a1, a2, a3;
-                            Code<ELEM, CT>::widen(wu[e], a0, a2);
-                            Code<ELEM, CT>::widen(vu[e], a1, a3);
+                            Code<MT, CT>::widen(wu[e], a0, a2);
+                            Code<MT, CT>::widen(vu[e], a1, a3);
 #pragma unroll
                             for (int nb = 0; nb < NB; nb++)
-                                mma16<ELEM>(x[kk][nb], a0, a1, a2, a3, qb[4 * c + e][nb]);
+                                mma16<MT>(x[kk][nb], a0, a1, a2, a3, qb[4 * c + e][nb]);
                         }
                     }
                 }
@@ -374,17 +438,17 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
             float alpha[NB][2];
 #pragma unroll
             for (int kk = 0; kk < C::BK / 16; kk++) {
-                float f0 = cscale, f1 = cscale;
+                float f0 = 1.f, f1 = 1.f;
                 if constexpr (C::Q8) {
-                    f0 *= __uint_as_float(lds4(sc + 16 + (kk * 16 + g) * 4));
-                    f1 *= __uint_as_float(lds4(sc + 16 + (kk * 16 + g + 8) * 4));
+                    f0 = __uint_as_float(lds4(sc + 16 + (kk * 16 + g) * 4));
+                    f1 = __uint_as_float(lds4(sc + 16 + (kk * 16 + g + 8) * 4));
                 }
 #pragma unroll
                 for (int nb = 0; nb < NB; nb++) {
-                    x[kk][nb][0] *= f0;
-                    x[kk][nb][1] *= f0;
-                    x[kk][nb][2] *= f1;
-                    x[kk][nb][3] *= f1;
+                    x[kk][nb][0] *= f0 * qscale[nb][0];
+                    x[kk][nb][1] *= f0 * qscale[nb][1];
+                    x[kk][nb][2] *= f1 * qscale[nb][0];
+                    x[kk][nb][3] *= f1 * qscale[nb][1];
                 }
                 if (edge) {
                     const uint32_t mask = PL > 1 && kk >= 2 ? there.y : there.x;
@@ -421,7 +485,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
                     }
                 }
             float vfix = 1.f;
-            if constexpr (C::Q8 && ELEM == kF16) {
+            if constexpr (C::Q8) {
                 float big = 0.f;
                 if (C::BK >= 32 || lane < C::BK)
                     big = __uint_as_float(lds4(sc + 16 + (C::BK + lane) * 4));
@@ -475,8 +539,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
                         p[2] *= v1;
                         p[3] *= v1;
                     }
-                    pb[nb][0] = transpose8(pack2<ELEM>(p[0], p[1]));
-                    pb[nb][1] = transpose8(pack2<ELEM>(p[2], p[3]));
+                    pb[nb][0] = transpose8(pack2<MT>(p[0], p[1]));
+                    pb[nb][1] = transpose8(pack2<MT>(p[2], p[3]));
                 }
 #pragma unroll
                 for (int c = 0; c < C::VCH; c++) {
@@ -503,17 +567,17 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
                             const uint32_t a3 = prmt(w[2][i4], w[3][i4], 0x7632);
 #pragma unroll
                             for (int nb = 0; nb < NB; nb++)
-                                mma16<ELEM>(o[c * C::VE / 2 + i4][nb], a0, a1, a2, a3, pb[nb]);
+                                mma16<MT>(o[c * C::VE / 2 + i4][nb], a0, a1, a2, a3, pb[nb]);
                         } else {
 #pragma unroll
                             for (int h = 0; h < 2; h++) {
                                 const uint32_t sel = h ? 0x7362 : 0x5140;
                                 uint32_t a0, a1, a2, a3;
-                                Code<ELEM, CT>::widen(prmt(w[0][i4], w[1][i4], sel), a0, a1);
-                                Code<ELEM, CT>::widen(prmt(w[2][i4], w[3][i4], sel), a2, a3);
+                                Code<MT, CT>::widen(prmt(w[0][i4], w[1][i4], sel), a0, a1);
+                                Code<MT, CT>::widen(prmt(w[2][i4], w[3][i4], sel), a2, a3);
 #pragma unroll
                                 for (int nb = 0; nb < NB; nb++)
-                                    mma16<ELEM>(o[c * C::VE / 2 + 2 * i4 + h][nb], a0, a1, a2, a3, pb[nb]);
+                                    mma16<MT>(o[c * C::VE / 2 + 2 * i4 + h][nb], a0, a1, a2, a3, pb[nb]);
                             }
                         }
                     }
@@ -548,32 +612,32 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
                     const int row = nb * 8 + 2 * t + (i & 1);
                     const int e = 2 * j + (i >> 1);  // column within the lane's pieces
                     const int d = (e / C::VE) * 8 * C::VE + g * C::VE + e % C::VE;
-                    if (row < rows) so[(warp * kRows + row) * (D + 4) + d] = o[j][nb][i] * UNSCALE;
+                    if (row < rows) so[(warp * kRows + row) * (D + 4) + d] = o[j][nb][i];
                 }
         __syncthreads();
         const bool whole = sg.parts == 1;
         float* slot = whole ? nullptr : part_slot(a, kRows, block, sg.part == 0);
-        for (int i = threadIdx.x; i < rows * D; i += kThreads) {
-            const int row = i / D, d = i - row * D;
+        constexpr int VL = D / 32;                   // columns per lane
+        for (int row = warp; row < rows; row += kWarps) {
             float mm = s_m[0][row];
 #pragma unroll
             for (int w = 1; w < kWarps; w++) mm = fmaxf(mm, s_m[w][row]);
             const float b = mm == -INFINITY ? 0.f : mm;
-            float ll = 0.f, v = 0.f;
+            float ll = 0.f, v[VL] = {};
 #pragma unroll
             for (int w = 0; w < kWarps; w++) {
                 const float f = ex2(s_m[w][row] - b);
                 ll += s_l[w][row] * f;
-                v += so[(w * kRows + row) * (D + 4) + d] * f;
+                float x[VL];
+                load_vec<VL>(x, so + (w * kRows + row) * (D + 4) + lane * VL);
+#pragma unroll
+                for (int i = 0; i < VL; i++) v[i] += x[i] * f;
             }
             if (whole) {
-                write_out<ELEM>(a, sg, row, d, mm, ll, v, s_bad);
+                write_out<ELEM, VL>(a, sg, row, lane * VL, mm, ll, v, s_bad);
             } else {
-                slot[2 * kRows + i] = v;
-                if (d == 0) {
-                    slot[2 * row] = mm;
-                    slot[2 * row + 1] = ll;
-                }
+                store_vec<VL>(slot + 2 * kRows + row * D + lane * VL, v);
+                if (lane == 0) *reinterpret_cast<float2*>(slot + 2 * row) = make_float2(mm, ll);
             }
         }
         bool final = whole;
@@ -585,21 +649,49 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
             final = s_last;
             if (final) {
                 __threadfence();
-                for (int i = threadIdx.x; i < rows * D; i += kThreads) {
-                    const int row = i / D, d = i - row * D;
-                    float mm = -INFINITY, ll = 0.f, v = 0.f;
-                    for (int p = 0; p < sg.parts; p++) {
-                        const float* ps = part_slot(a, kRows, sg.first + p, p == 0);
-                        const float pm = __ldcg(ps + 2 * row), pl = __ldcg(ps + 2 * row + 1);
-                        const float pv = __ldcg(ps + 2 * kRows + i);
-                        const float nm = fmaxf(mm, pm);
+                for (int row = warp; row < rows; row += kWarps) {
+                    float mm = -INFINITY, ll = 0.f, v[VL] = {};
+                    for (int p0 = 0; p0 < sg.parts; p0 += 32) {
+                        // lane i: maximum and sum of part p0 + i
+                        const int np = min(32, sg.parts - p0);
+                        float2 ml = make_float2(-INFINITY, 0.f);
+                        if (lane < np)
+                            ml = __ldcg(reinterpret_cast<const float2*>(
+                                part_slot(a, kRows, sg.first + p0 + lane, p0 + lane == 0) + 2 * row));
+                        float nm = ml.x;
+#pragma unroll
+                        for (int o2 = 16; o2 > 0; o2 >>= 1)
+                            nm = fmaxf(nm, __shfl_xor_sync(0xffffffffu, nm, o2));
+                        nm = fmaxf(nm, mm);
                         const float b = nm == -INFINITY ? 0.f : nm;
-                        const float f0 = ex2(mm - b), f1 = ex2(pm - b);
-                        ll = ll * f0 + pl * f1;
-                        v = v * f0 + pv * f1;
+                        const float f = ex2(ml.x - b), back = ex2(mm - b);
+                        float sum = ml.y * f;
+#pragma unroll
+                        for (int o2 = 16; o2 > 0; o2 >>= 1)
+                            sum += __shfl_xor_sync(0xffffffffu, sum, o2);
+                        ll = ll * back + sum;
+#pragma unroll
+                        for (int i = 0; i < VL; i++) v[i] *= back;
                         mm = nm;
+                        for (int p = 0; p < np; p += 8) {
+                            float x[8][VL];
+#pragma unroll
+                            for (int u = 0; u < 8; u++)
+                                if (p + u < np)
+                                    load_vec_cg<VL>(x[u], part_slot(a, kRows, sg.first + p0 + p + u,
+                                                                    p0 + p + u == 0) +
+                                                              2 * kRows + row * D + lane * VL);
+#pragma unroll
+                            for (int u = 0; u < 8; u++) {
+                                const float fu = __shfl_sync(0xffffffffu, f, (p + u) & 31);
+                                if (p + u < np) {
+#pragma unroll
+                                    for (int i = 0; i < VL; i++) v[i] = fmaf(x[u][i], fu, v[i]);
+                                }
+                            }
+                        }
                     }
-                    write_out<ELEM>(a, sg, row, d, mm, ll, v, s_bad);
+                    write_out<ELEM, VL>(a, sg, row, lane * VL, mm, ll, v, s_bad);
                 }
             }
         }
@@ -608,6 +700,33 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
         fence_async_smem();                          // the rings are TMA's again
         __syncthreads();
     }
+}
+
+// row blocks of 8: those of the longest chunk, as the caller tells it
+int row_blocks(const PagedAttn& a) {
+    const long long rows = (long long)std::max(1, a.max_q) * a.group;
+    return (int)std::min<long long>((rows + 7) / 8, kMaxNB);
+}
+
+// How many pieces the work is cut into: those that start together, fewer when
+// the page table cannot hold that much work, and the small ones behind them.
+struct Pieces {
+    int blocks, extra;
+};
+int most_together(const PagedAttn& a) {
+    return std::min((row_blocks(a) == 1 ? 3 : 2) * num_sms(), kMaxBlocks / (1 + kExtra));
+}
+Pieces pieces(const PagedAttn& a) {
+    const int nb = row_blocks(a), together = most_together(a);
+    const int step = kWarps * 4096 / (a.c.dim * (a.type >= kI8 ? 1 : 2));
+    const long long keys = (long long)a.tpages * a.c.ps;
+    const long long tile_tokens = 8 * nb / a.group;
+    const long long tiles = (a.total_q + tile_tokens - 1) / tile_tokens + a.batch;
+    const long long most = std::max(1LL, (keys + step - 1) / step) * std::min<long long>(tiles, 1 << 20) *
+                           a.c.heads;
+    if (most <= (long long)together * 2 * kLeast)
+        return {(int)std::max(1LL, (most + kLeast - 1) / kLeast), 0};
+    return {together, kExtra * together};
 }
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
@@ -664,21 +783,16 @@ int launch(const PagedAttn& a, cudaStream_t s) {
         if (e != cudaSuccess) return (int)e;
         attr_set.fetch_or(bit);
     }
-    const SchedShape shape{C::ROWS / a.group, kWarps * C::BK, 2};
+    const Pieces pc = pieces(a);
+    const SchedShape shape{C::ROWS / a.group, kWarps * C::BK, kLeast, pc.blocks, pc.extra, kShare};
     int box = 8;                                     // tokens of a page side by side
     while (box < C::BK && a.c.ps % (2 * box) == 0) box *= 2;
     CUtensorMap tk, tv;
     if (!cache_map(&tk, a, a.c.k, C::RB, box) || !cache_map(&tv, a, a.c.v, C::RB, box)) return 1;
-    kern<<<std::min(C::PER_SM * num_sms(), kMaxBlocks), kThreads, C::SMEM, s>>>(tk, tv, a, shape, box);
+    kern<<<pc.blocks + pc.extra, kThreads, C::SMEM, s>>>(tk, tv, a, shape, box);
     const cudaError_t e = cudaGetLastError();
     if (e == cudaSuccess) note_launch();
     return e == cudaSuccess ? 0 : (int)e;
-}
-
-// row blocks of 8: those of the longest chunk, as the caller tells it
-int row_blocks(const PagedAttn& a) {
-    const long long rows = (long long)std::max(1, a.max_q) * a.group;
-    return (int)std::min<long long>((rows + 7) / 8, kMaxNB);
 }
 
 template <int D, int ELEM, int CT>
@@ -700,9 +814,9 @@ int launch_dim(const PagedAttn& a, cudaStream_t s) {
 int decode_max_rows() { return 8 * kMaxNB; }
 
 size_t paged_decode_workspace(const PagedAttn& a) {
-    const int nb = row_blocks(a), per_sm = nb == 1 ? 3 : 2;
-    const int blocks = std::min(per_sm * num_sms(), kMaxBlocks);
-    return kCounterBytes + 2ull * blocks * slot_floats(8 * nb, a.c.dim) * sizeof(float);
+    // (not by the length of the page table, which may grow between calls)
+    return kCounterBytes +
+           2ull * (1 + kExtra) * most_together(a) * slot_floats(8 * row_blocks(a), a.c.dim) * sizeof(float);
 }
 
 int paged_decode(const PagedAttn& a, cudaStream_t s) {

@@ -25,15 +25,20 @@ __device__ __forceinline__ float lse_of(float m2, float l) {
     return l == 0.f ? -INFINITY : m2 * 0.6931471805599453f + logf(l);
 }
 
-// element d of a row, v the unnormalised value, m2 and l the row's maximum
-// (log2 units) and sum
-template <int ELEM>
+// columns d .. d + N - 1 of a row, v the unnormalised values, m2 and l the
+// row's maximum (log2 units) and sum
+template <int ELEM, int N>
 __device__ __forceinline__ void write_out(const PagedAttn& a, const Segment& g, int row, int d,
-                                          float m2, float l, float v, int* bad) {
+                                          float m2, float l, const float (&v)[N], int* bad) {
     const RowPlace r = row_place(a, g, row);
-    const float x = l == 0.f ? 0.f : v / l;
-    if (!isfinite(x)) bad[row] = 1;
-    store_as(a.o + (r.token * a.orow + r.head * a.oh + d) * 2, ELEM, x);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    char* o = a.o + (r.token * a.orow + r.head * a.oh + d) * 2;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const float x = v[i] * inv;
+        if (!isfinite(x)) bad[row] = 1;
+        store_as(o + 2 * i, ELEM, x);
+    }
     if (d == 0 && a.lse) a.lse[r.head * a.lh + r.token] = lse_of(m2, l);
 }
 

@@ -3,10 +3,13 @@
 // A unit is a tile of query rows of one sequence and KV head; its steps are
 // the key tiles that its rows see (one at least, so that rows which see
 // nothing are written too).  All steps of all units, in the order sequence,
-// head, tile, key, form one line, and block x takes the x-th equal piece of
-// it.  Lengths live on the device, so every block works its piece out from
-// them: nothing is planned on the host, a ragged batch is as even as a
-// regular one, and a graph replays with new lengths.
+// head, tile, key, form one line, and block x takes the x-th piece of it:
+// `blocks` equal pieces that start together, and, where blocks of equal work
+// do not end together, `extra` small ones behind them that the hardware
+// starts wherever a block has ended.  Lengths live on the device, so every
+// block works its piece out from them: nothing is planned on the host, a
+// ragged batch is as even as a regular one, and a graph replays with new
+// lengths.  (Positions are 32 bits: 2^32 steps are minutes of work.)
 //
 // A unit that spans several blocks is joined by whichever of them finishes
 // last: each leaves its unnormalised O with the maximum and the sum of every
@@ -25,7 +28,9 @@ namespace zl {
 struct SchedShape {
     int tokens;          // query tokens per tile
     int step;            // keys per step
-    int least;           // steps per block, at least
+    int least;           // steps per piece, at least
+    int blocks, extra;   // pieces of the first and of the second kind
+    int share;           // 256ths of the line that the first kind takes
 };
 
 // one block's piece of one unit
@@ -49,61 +54,91 @@ __device__ __forceinline__ int tile_steps(const PagedAttn& a, const SchedShape& 
 }
 
 // steps of all tiles of one head of a sequence
-__device__ __forceinline__ long long head_steps(const PagedAttn& a, const SchedShape& h,
-                                                const SeqInfo& q) {
+__device__ __forceinline__ unsigned head_steps(const PagedAttn& a, const SchedShape& h,
+                                               const SeqInfo& q) {
+    if (q.n <= h.tokens) return q.n ? tile_steps(a, h, q, 0) : 0;
     const int tiles = (q.n + h.tokens - 1) / h.tokens;
-    if (!a.causal) return tiles ? (long long)tiles * tile_steps(a, h, q, 0) : 0;
-    long long sum = 0;
+    if (!a.causal) return (unsigned)tiles * tile_steps(a, h, q, 0);
+    unsigned sum = 0;
     for (int t = 0; t < tiles; t++) sum += tile_steps(a, h, q, t);
     return sum;
+}
+
+// inclusive sum over the lanes
+__device__ __forceinline__ unsigned lane_sums(unsigned v) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned x = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += x;
+    }
+    return v;
 }
 
 // Walks a block's piece.  Every warp keeps one of its own (the search runs
 // across the lanes; all lanes hold the same state afterwards).
 struct Walker {
-    long long pos, end, per, begin;      // on the line; begin: of the unit
+    unsigned pos, end, begin;            // on the line; begin: of the unit
+    unsigned big, small, turn;           // piece sizes, and where the small ones start
     SeqInfo q;
-    int s, head, tile, steps;
+    int s, head, tile;
+    unsigned steps;
 
     __device__ __forceinline__ void enter(const PagedAttn& a, const SchedShape& h) {
         steps = tile_steps(a, h, q, tile);
     }
 
-    __device__ void start(const PagedAttn& a, const SchedShape& h, int block, int blocks) {
+    // the piece that holds a position
+    __device__ __forceinline__ unsigned piece_of(const SchedShape& h, unsigned p) const {
+        return p < turn ? p / big : h.blocks + (p - turn) / small;
+    }
+
+    __device__ void start(const PagedAttn& a, const SchedShape& h, int block) {
         const int lane = threadIdx.x & 31;
-        long long mine = 0;
-        for (int b = lane; b < a.batch; b += 32) mine += head_steps(a, h, seq_info(a, b));
+        // lane l sums sequences [l * each, (l + 1) * each)
+        const int each = (a.batch + 31) / 32;
+        unsigned mine = 0;
+        for (int i = 0; i < each; i++) {
+            const int b = lane * each + i;
+            if (b < a.batch) mine += head_steps(a, h, seq_info(a, b));
+        }
         mine *= a.c.heads;
-        long long total = mine;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        per = max((total + blocks - 1) / blocks, (long long)h.least);
-        pos = min(total, block * per);
-        end = min(total, pos + per);
+        const unsigned sum = lane_sums(mine);
+        const unsigned total = __shfl_sync(0xffffffffu, sum, 31);
+        const unsigned fair = (total + h.blocks - 1) / h.blocks;
+        big = max((unsigned)h.least, h.extra ? (fair * h.share + 255) / 256 : fair);
+        turn = min(total, big * h.blocks);
+        small = h.extra ? max((unsigned)h.least, (total - turn + h.extra - 1) / h.extra) : 1;
+        if (block < h.blocks) {
+            pos = min(turn, block * big);
+            end = min(turn, pos + big);
+        } else {
+            pos = min(total, turn + (block - h.blocks) * small);
+            end = min(total, pos + small);
+        }
         if (pos >= end) return;
-        // the sequence that holds pos: running sums over 32 sequences at a time
-        long long base = 0;
-        for (int b0 = 0;; b0 += 32) {
-            const int b = b0 + lane;
-            long long v = a.batch <= 32 ? mine
-                        : b < a.batch ? head_steps(a, h, seq_info(a, b)) * a.c.heads : 0;
-            long long sum = v;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long x = __shfl_up_sync(0xffffffffu, sum, o);
-                if (lane >= o) sum += x;
+        // the lane whose sequences hold pos, then the sequence
+        int l = __ffs(__ballot_sync(0xffffffffu, sum > pos)) - 1;
+        unsigned base = __shfl_sync(0xffffffffu, sum - mine, l);
+        s = l * each;
+        if (each > 1) {
+            for (int b0 = l * each;; b0 += 32) {
+                const int b = b0 + lane;
+                const unsigned v = b < min(a.batch, (l + 1) * each)
+                                       ? head_steps(a, h, seq_info(a, b)) * a.c.heads : 0;
+                const unsigned x = lane_sums(v);
+                const unsigned past = __ballot_sync(0xffffffffu, base + x > pos);
+                if (past) {
+                    const int f = __ffs(past) - 1;
+                    s = b0 + f;
+                    base += __shfl_sync(0xffffffffu, x - v, f);
+                    break;
+                }
+                base += __shfl_sync(0xffffffffu, x, 31);
             }
-            const unsigned past = __ballot_sync(0xffffffffu, base + sum > pos);
-            if (past) {
-                const int l = __ffs(past) - 1;
-                s = b0 + l;
-                base += __shfl_sync(0xffffffffu, sum - v, l);
-                break;
-            }
-            base += __shfl_sync(0xffffffffu, sum, 31);
         }
         q = seq_info(a, s);
-        const long long hs = head_steps(a, h, q);
+        const unsigned hs = head_steps(a, h, q);
         head = (int)((pos - base) / hs);
         begin = base + head * hs;
         tile = 0;
@@ -124,18 +159,18 @@ struct Walker {
         g.q = q;
         g.i0 = tile * h.tokens;
         g.ni = min(h.tokens, q.n - g.i0);
-        const int st0 = (int)(pos - begin);
-        const int st1 = (int)min((long long)steps, end - begin);
+        const unsigned st0 = pos - begin;
+        const unsigned st1 = min(steps, end - begin);
         const int e = tile_end(a, q, g.i0 + g.ni);
-        g.k0 = min(e, st0 * h.step);
-        g.k1 = (int)min((long long)e, (long long)st1 * h.step);
+        g.k0 = (int)min((unsigned)e, st0 * h.step);
+        g.k1 = (int)min((unsigned)e, st1 * h.step);
         if (st0 == 0 && st1 == steps) {
             g.parts = 1;
             g.part = 0;
             g.first = block;
         } else {
-            g.first = (int)(begin / per);
-            g.parts = (int)((begin + steps - 1) / per) - g.first + 1;
+            g.first = (int)piece_of(h, begin);
+            g.parts = (int)piece_of(h, begin + steps - 1) - g.first + 1;
             g.part = block - g.first;
         }
         pos = begin + st1;
@@ -157,7 +192,7 @@ struct Walker {
 
 // ---- the workspace --------------------------------------------------------------
 
-constexpr int kMaxBlocks = 1024;                 // two counters each
+constexpr int kMaxBlocks = 4096;                 // pieces; two counters each
 constexpr size_t kCounterBytes = 2 * kMaxBlocks * sizeof(int);
 
 // floats of one slot: (maximum, sum) of every row, then O
