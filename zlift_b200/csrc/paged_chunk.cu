@@ -748,7 +748,7 @@ int launch(const PagedAttn& a, cudaStream_t s) {
     using C = PCfg<D, (CT >= kI8)>;
     ChunkShape shape;
     shape.tile_tokens = BQ / a.group;
-    shape.sched = SchedShape{2 * shape.tile_tokens, BKEY, 2, chunk_blocks(), 0, 256};
+    shape.sched = SchedShape{2 * shape.tile_tokens, BKEY, 2, chunk_blocks()};
     shape.box = 8;
     while (shape.box < BKEY && a.c.ps % (2 * shape.box) == 0) shape.box *= 2;
     CUtensorMap tq, tk, tv;
@@ -791,7 +791,7 @@ int launch_dim(const PagedAttn& a, cudaStream_t s) {
 
 }  // namespace
 
-int chunk_blocks() { return std::min(num_sms(), kMaxBlocks); }
+int chunk_blocks() { return std::min(num_sms(), kMaxPieces); }
 
 size_t paged_chunk_workspace(const PagedAttn& a) {
     return kCounterBytes + 4ull * chunk_blocks() * slot_floats(BQ, a.c.dim) * sizeof(float);

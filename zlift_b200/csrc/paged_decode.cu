@@ -48,9 +48,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMaxNB = 3;
-constexpr int kLeast = 2;                // steps of a piece, at least
-constexpr int kExtra = 2;                // small pieces for each large one
-constexpr int kShare = 200;              // 256ths of the work in large pieces
+constexpr int kLeast = 2;                // blocks of keys of a piece, at least
 constexpr float kLazy = 6.f;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -72,9 +70,7 @@ struct DCfg {
     static constexpr int RING = STAGES * 8192;
     static constexpr int SIDE = (Q8 ? 2 * BK * 4 : 0) + 16;  // scales, keys there; per stage
     static constexpr int SIDE_OFF = kWarps * RING;
-    static constexpr int JOIN = kWarps * ROWS * (D + 4) * 4;
     static constexpr int SMEM = SIDE_OFF + kWarps * STAGES * SIDE + 1024;
-    static_assert(JOIN <= SIDE_OFF, "the join reuses the rings");
     static_assert(NT * KCH == 8 && BK / 4 * VCH * VP == 128, "a block is 8 KB");
 };
 
@@ -135,33 +131,6 @@ __device__ __forceinline__ void copy_wait() {
     asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory");
 }
 
-// N (2 or 4) floats at an address aligned for them
-template <int N>
-__device__ __forceinline__ void load_vec(float (&x)[N], const float* p) {
-    if constexpr (N == 4) {
-        const float4 v = *reinterpret_cast<const float4*>(p);
-        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-    } else {
-        const float2 v = *reinterpret_cast<const float2*>(p);
-        x[0] = v.x; x[1] = v.y;
-    }
-}
-template <int N>
-__device__ __forceinline__ void load_vec_cg(float (&x)[N], const float* p) {
-    if constexpr (N == 4) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(p));
-        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-    } else {
-        const float2 v = __ldcg(reinterpret_cast<const float2*>(p));
-        x[0] = v.x; x[1] = v.y;
-    }
-}
-template <int N>
-__device__ __forceinline__ void store_vec(float* p, const float (&x)[N]) {
-    if constexpr (N == 4) *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-    else *reinterpret_cast<float2*>(p) = make_float2(x[0], x[1]);
-}
-
 __device__ __forceinline__ uint4 lds16(uint32_t a) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
@@ -205,24 +174,113 @@ __device__ __forceinline__ float halve_row(uint32_t (&qb)[D / 16][NB][2], int nb
     return __uint_as_float((uint32_t)(127 + e) << 23);
 }
 
+// Sums a unit's parts, in key order, into this warp's registers.
+template <int D, int NB>
+__device__ __forceinline__ void join_parts(const PagedAttn& a, const Segment& sg,
+                                           float (&o)[D / 16][NB][4], float (&m)[NB][2],
+                                           float (&l)[NB][2]) {
+    const int lane = threadIdx.x & 31, t = lane & 3;
+    auto slot = [&](int p) { return part_slot(a, 8 * NB, sg.first + p, p == 0); };
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {
+        // maxima first (a load each, all independent), then sums, then O
+        float mm[2] = {-INFINITY, -INFINITY};
+#pragma unroll 4
+        for (int p = 0; p < sg.parts; p++) {
+            const float4 ml = __ldcg(reinterpret_cast<const float4*>(slot(p)) + nb * 4 + t);
+            mm[0] = fmaxf(mm[0], ml.x);
+            mm[1] = fmaxf(mm[1], ml.z);
+        }
+        m[nb][0] = mm[0];
+        m[nb][1] = mm[1];
+        const float b0 = mm[0] == -INFINITY ? 0.f : mm[0], b1 = mm[1] == -INFINITY ? 0.f : mm[1];
+        l[nb][0] = l[nb][1] = 0.f;
+#pragma unroll
+        for (int j = 0; j < D / 16; j++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[j][nb][i] = 0.f;
+#pragma unroll 2
+        for (int p = 0; p < sg.parts; p++) {
+            const float4 ml = __ldcg(reinterpret_cast<const float4*>(slot(p)) + nb * 4 + t);
+            const float4* so = reinterpret_cast<const float4*>(slot(p) + 16 * NB) + lane;
+            float4 v[D / 16];
+#pragma unroll
+            for (int j = 0; j < D / 16; j++) v[j] = __ldcg(so + (nb * (D / 16) + j) * 32);
+            const float f0 = ex2(ml.x - b0), f1 = ex2(ml.z - b1);
+            l[nb][0] = fmaf(ml.y, f0, l[nb][0]);
+            l[nb][1] = fmaf(ml.w, f1, l[nb][1]);
+#pragma unroll
+            for (int j = 0; j < D / 16; j++) {
+                o[j][nb][0] = fmaf(v[j].x, f0, o[j][nb][0]);
+                o[j][nb][1] = fmaf(v[j].y, f1, o[j][nb][1]);
+                o[j][nb][2] = fmaf(v[j].z, f0, o[j][nb][2]);
+                o[j][nb][3] = fmaf(v[j].w, f1, o[j][nb][3]);
+            }
+        }
+    }
+}
+
+// Normalises and stores a tile's rows, and redoes those a masked key spoilt.
+template <int D, int ELEM, int CT, int NB>
+__device__ __forceinline__ void finish_rows(const PagedAttn& a, const Segment& sg, int rows,
+                                            const float (&o)[D / 16][NB][4], const float (&m)[NB][2],
+                                            const float (&l)[NB][2]) {
+    using C = DCfg<D, CT, NB>;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const bool vec = ((reinterpret_cast<uintptr_t>(a.o) | (a.orow * 2) | (a.oh * 2)) & 15) == 0;
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int row = nb * 8 + 2 * t + e;
+            const bool live = row < rows;
+            const RowPlace pl = row_place(a, sg, live ? row : 0);
+            const float inv = l[nb][e] == 0.f ? 0.f : 1.f / l[nb][e];
+            char* orow = a.o + (pl.token * a.orow + pl.head * a.oh) * 2;
+            float z = 0.f;
+#pragma unroll
+            for (int c = 0; c < D / 64; c++) {       // 8 columns that follow one another
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float x = o[4 * c + i][nb][e] * inv, y = o[4 * c + i][nb][2 + e] * inv;
+                    z = fmaf(x, 0.f, fmaf(y, 0.f, z));       // NaN once one is not finite
+                    w[i] = pack2<ELEM>(x, y);
+                }
+                const int d = C::VE == 8 ? c * 64 + g * 8 : g * 16 + c * 8;
+                char* p = orow + d * 2;
+                if (live && vec) {
+                    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+                } else if (live) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+                }
+            }
+            if (live && g == 0 && a.lse) a.lse[pl.head * a.lh + pl.token] = lse_of(m[nb][e], l[nb][e]);
+            const unsigned bad = __ballot_sync(0xffffffffu, live && z != 0.f);
+            if (bad)
+                for (int i = 0; i < 4; i++)
+                    if ((bad >> i) & 0x11111111u) repair_row(a, sg, nb * 8 + 2 * i + e);
+        }
+}
+
 template <int D, int ELEM, int CT, int NB>
 __global__ void __launch_bounds__(kThreads, DCfg<D, CT, NB>::PER_SM)
 paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
                     const __grid_constant__ CUtensorMap tmV,
                     const __grid_constant__ PagedAttn a, const SchedShape shape, const int box) {
     using C = DCfg<D, CT, NB>;
-    constexpr int kRows = C::ROWS, kStages = C::STAGES;
+    constexpr int kStages = C::STAGES;
     constexpr int MT = C::Q8 ? kF16 : ELEM;          // type of the products' operands
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     __shared__ uint64_t s_full[kWarps][kStages];
     __shared__ int s_abort;
-    __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
-    __shared__ int s_last, s_bad[kRows];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
-    const int block = blockIdx.x;
+    const int piece = blockIdx.x * kWarps + warp;
     uint8_t* ring = smem + warp * C::RING;
     const uint32_t side = smem_u32(smem + C::SIDE_OFF) + warp * kStages * C::SIDE;
     const float cscale = a.scale * kLog2e;
@@ -232,7 +290,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
         s_abort = 0;
         fence_mbar_init();
     }
-    __syncthreads();
+    __syncthreads();                                 // from here on every warp is alone
     // where this lane's operands sit in a stage: K pieces t and t + 4 of row g,
     // V piece g of rows 2t and 2t + 1 (swizzled as TMA stores them)
     const uint32_t k_even = C::RB == 128 ? g * 128 + ((t ^ g) << 4) : g * 64 + ((t ^ (g >> 1)) << 4);
@@ -247,85 +305,92 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
     bool alive = true;
 
     Walker walk;
-    walk.start(a, shape, block);
-    Segment sg;
-    while (walk.next(a, shape, block, sg)) {
-        const int rows = sg.ni * a.group;
-        const float* ksb = a.c.ks + sg.head * a.c.shead;
-        const float* vsb = a.c.vs + sg.head * a.c.shead;
-        const int* table = a.table + sg.s * a.tstride;
-        const int stride = kWarps * C::BK;
-        const int first = sg.k0 + warp * C::BK;
-        const int mine = alive && sg.k1 > first ? (sg.k1 - first + stride - 1) / stride : 0;
+    walk.start(a, shape, piece);
+    Segment sg, nx;
+    bool more = walk.next(a, shape, piece, sg);
 
-        // ---- loads: block i into stage i % kStages
-        constexpr int PL = C::BK > 32 ? 2 : 1;       // keys per lane
-        int page[PL];
-        auto fetch_pages = [&](int i) {
+    // ---- loads: block i of a segment into the next stage
+    constexpr int PL = C::BK > 32 ? 2 : 1;           // keys per lane
+    auto blocks_of = [&](const Segment& z) { return alive ? (z.k1 - z.k0 + C::BK - 1) / C::BK : 0; };
+    auto page_at = [&](const Segment& z, int i, int h) {     // -2: past the end
+        const int key = z.k0 + i * C::BK + h * 32 + lane;
+        return (C::BK >= 32 || lane < C::BK) && key < z.k1
+                   ? __ldg(a.table + z.s * a.tstride + a.c.by_ps.div(key)) : -2;
+    };
+    auto load_block = [&](const Segment& z, int i, const int (&page)[PL]) {
+        const uint32_t stage = filled % kStages;
+        filled++;
+        uint32_t there[PL];
 #pragma unroll
-            for (int h = 0; h < PL; h++) {
-                const int key = first + i * stride + h * 32 + lane;
-                page[h] = -2;                        // past the end
-                if ((C::BK >= 32 || lane < C::BK) && key < sg.k1)
-                    page[h] = __ldg(table + a.c.by_ps.div(key));
-            }
-        };
-        auto load_block = [&](int i) {
-            const uint32_t stage = filled % kStages;
-            filled++;
-            uint32_t there[PL];
-#pragma unroll
-            for (int h = 0; h < PL; h++) {
-                const bool ok = (unsigned)page[h] < (unsigned)a.c.pages;
-                if (!ok && page[h] != -2) note_bad_index();
-                there[h] = __ballot_sync(0xffffffffu, ok);
-                if constexpr (C::Q8) {
-                    if (C::BK >= 32 || lane < C::BK) {
-                        const int key = first + i * stride + h * 32 + lane;
-                        const int off = key - (int)a.c.by_ps.div(key) * a.c.ps;
-                        const long long sat = ok ? page[h] * a.c.spage + off : 0;
-                        const uint32_t d = side + stage * C::SIDE + 16 + (h * 32 + lane) * 4;
-                        copy_async4(d, ksb + sat, ok);
-                        copy_async4(d + C::BK * 4, vsb + sat, ok);
-                    }
+        for (int h = 0; h < PL; h++) {
+            const bool ok = (unsigned)page[h] < (unsigned)a.c.pages;
+            if (!ok && page[h] != -2) note_bad_index();
+            there[h] = __ballot_sync(0xffffffffu, ok);
+            if constexpr (C::Q8) {
+                if (C::BK >= 32 || lane < C::BK) {
+                    const int key = z.k0 + i * C::BK + h * 32 + lane;
+                    const int off = key - (int)a.c.by_ps.div(key) * a.c.ps;
+                    const long long sat = (ok ? page[h] * a.c.spage + off : 0) + z.head * a.c.shead;
+                    const uint32_t d = side + stage * C::SIDE + 16 + (h * 32 + lane) * 4;
+                    copy_async4(d, a.c.ks + sat, ok);
+                    copy_async4(d + C::BK * 4, a.c.vs + sat, ok);
                 }
             }
-            if (lane == 0) {
-                asm volatile("st.shared.v2.u32 [%0], {%1,%2};" :: "r"(side + stage * C::SIDE),
-                             "r"(there[0]), "r"(there[PL - 1]) : "memory");
-                mbar_expect_tx(&s_full[warp][stage], 8192);
-            }
-            __syncwarp();
-            const int r = box_row * box;
-            int pg = __shfl_sync(0xffffffffu, page[0], r & 31);
-            if constexpr (PL > 1) {
-                const int p1 = __shfl_sync(0xffffffffu, page[1], r & 31);
-                if (r >= 32) pg = p1;
-            }
-            if (box_mine) {
-                const int key = first + i * stride + r;
-                const int off = key - (int)a.c.by_ps.div(key) * a.c.ps;
-                // a page that is not there, or not wanted, is asked for out of
-                // range and arrives as zeros
-                if ((unsigned)pg >= (unsigned)a.c.pages) pg = a.c.pages;
-                tma_load_4d(ring + stage * 8192 + box_kv * 4096 + box_col * (C::BK * C::RB) + r * C::RB,
-                            box_kv ? &tmV : &tmK, &s_full[warp][stage], box_col * (128 / C::EB), off,
-                            sg.head, pg);
-            }
-        };
-
-        fetch_pages(0);
+        }
+        if (lane == 0) {
+            asm volatile("st.shared.v2.u32 [%0], {%1,%2};" :: "r"(side + stage * C::SIDE),
+                         "r"(there[0]), "r"(there[PL - 1]) : "memory");
+            mbar_expect_tx(&s_full[warp][stage], 8192);
+        }
+        __syncwarp();
+        const int r = box_row * box;
+        int pg = __shfl_sync(0xffffffffu, page[0], r & 31);
+        if constexpr (PL > 1) {
+            const int p1 = __shfl_sync(0xffffffffu, page[1], r & 31);
+            if (r >= 32) pg = p1;
+        }
+        if (box_mine) {
+            const int key = z.k0 + i * C::BK + r;
+            const int off = key - (int)a.c.by_ps.div(key) * a.c.ps;
+            // a page that is not there, or not wanted, is asked for out of
+            // range and arrives as zeros
+            if ((unsigned)pg >= (unsigned)a.c.pages) pg = a.c.pages;
+            tma_load_4d(ring + stage * 8192 + box_kv * 4096 + box_col * (C::BK * C::RB) + r * C::RB,
+                        box_kv ? &tmV : &tmK, &s_full[warp][stage], box_col * (128 / C::EB), off,
+                        z.head, pg);
+        }
+    };
+    int page[kStages][PL];                           // of a segment's first blocks
+    auto first_pages = [&](const Segment& z) {
+#pragma unroll
+        for (int i = 0; i < kStages; i++)
+#pragma unroll
+            for (int h = 0; h < PL; h++) page[i][h] = page_at(z, i, h);
+    };
+    auto first_blocks = [&](const Segment& z) {
+        const int n = blocks_of(z);
 #pragma unroll
         for (int i = 0; i < kStages - 1; i++) {
-            if (i < mine) load_block(i);
-            fetch_pages(i + 1);
+            if (i < n) load_block(z, i, page[i]);
             copy_commit();
         }
+    };
+    if (more) {
+        first_pages(sg);
+        first_blocks(sg);
+    }
+
+    while (more) {
+        const int rows = sg.ni * a.group;
+        const int mine = blocks_of(sg);
+        int ahead[PL];                               // pages of the next block to load
+#pragma unroll
+        for (int h = 0; h < PL; h++) ahead[h] = page[kStages - 1][h];
 
         // ---- queries: row nb * 8 + g, dim permuted as the K pieces are
         uint32_t qb[D / 16][NB][2];
-        float qscale[NB][2];                         // of rows nb*8 + 2t, + 1 (8-bit caches)
-        int lim[NB][2];                              // keys that rows nb*8 + 2t, + 1 see
+        float qscale[NB][2];                         // of rows nb*8 + 2t, + 1
+        int lim[NB][2];                              // keys that they see
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) {
             const int row = nb * 8 + g;
@@ -371,12 +436,13 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
             base[nb][0] = base[nb][1] = 0.f;
             l[nb][0] = l[nb][1] = 0.f;
         }
-        float vmost = 0.f, vpow = 1.f, lpow = 0.f;   // fp16: see v_power
+        float vmost = 0.f, vpow = 1.f, lpow = 0.f;   // 8 bit: see v_power
 
         for (int i = 0; i < mine; i++) {
             __syncwarp();                            // the stage to fill is no longer read
-            if (i + kStages - 1 < mine) load_block(i + kStages - 1);
-            fetch_pages(i + kStages);
+            if (i + kStages - 1 < mine) load_block(sg, i + kStages - 1, ahead);
+#pragma unroll
+            for (int h = 0; h < PL; h++) ahead[h] = page_at(sg, i + kStages, h);
             copy_commit();
             const uint32_t stage = used % kStages;
             const uint32_t st = smem_u32(ring) + stage * 8192, sc = side + stage * C::SIDE;
@@ -384,7 +450,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
             alive = __all_sync(0xffffffffu, mbar_wait(&s_full[warp][stage], (used / kStages) & 1, &s_abort));
             if (!alive) break;
             used++;
-            const int kb = first + i * stride;
+            const int kb = sg.k0 + i * C::BK;
             // V rows past the keys, in a box that is partly wanted, may hold
             // anything: 0 times them must be 0
             const int left = sg.k1 - kb;
@@ -586,119 +652,55 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
         }
         copy_wait<0>();
 
-        // ---- join the warps: maxima and sums, then O through shared memory
+        // ---- the next segment's pages are on their way while this one ends
+        more = walk.next(a, shape, piece, nx);
+        if (more) first_pages(nx);
 #pragma unroll
         for (int nb = 0; nb < NB; nb++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                float sum = l[nb][e];
-                sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-                if (g == 0) {
-                    s_m[warp][nb * 8 + 2 * t + e] = m[nb][e] - lpow;
-                    s_l[warp][nb * 8 + 2 * t + e] = sum;
-                }
+                l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], 4);
+                l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], 8);
+                l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], 16);
+                m[nb][e] -= lpow;                    // log2 units, of O and l alike
             }
-        if (threadIdx.x < kRows) s_bad[threadIdx.x] = 0;
-        __syncthreads();                             // also: every ring is drained
-        float* so = reinterpret_cast<float*>(smem);  // [warp][row][D + 4]
+        bool final = sg.parts == 1;
+        if (!final) {
+            float* slot = part_slot(a, C::ROWS, piece, sg.part == 0);
+            if (g == 0) {
 #pragma unroll
-        for (int j = 0; j < D / 16; j++)
+                for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++)
+                        reinterpret_cast<float2*>(slot)[nb * 8 + 2 * t + e] = make_float2(m[nb][e], l[nb][e]);
+            }
+            float4* so = reinterpret_cast<float4*>(slot + 2 * C::ROWS) + lane;
 #pragma unroll
             for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int row = nb * 8 + 2 * t + (i & 1);
-                    const int e = 2 * j + (i >> 1);  // column within the lane's pieces
-                    const int d = (e / C::VE) * 8 * C::VE + g * C::VE + e % C::VE;
-                    if (row < rows) so[(warp * kRows + row) * (D + 4) + d] = o[j][nb][i];
-                }
-        __syncthreads();
-        const bool whole = sg.parts == 1;
-        float* slot = whole ? nullptr : part_slot(a, kRows, block, sg.part == 0);
-        constexpr int VL = D / 32;                   // columns per lane
-        for (int row = warp; row < rows; row += kWarps) {
-            float mm = s_m[0][row];
-#pragma unroll
-            for (int w = 1; w < kWarps; w++) mm = fmaxf(mm, s_m[w][row]);
-            const float b = mm == -INFINITY ? 0.f : mm;
-            float ll = 0.f, v[VL] = {};
-#pragma unroll
-            for (int w = 0; w < kWarps; w++) {
-                const float f = ex2(s_m[w][row] - b);
-                ll += s_l[w][row] * f;
-                float x[VL];
-                load_vec<VL>(x, so + (w * kRows + row) * (D + 4) + lane * VL);
-#pragma unroll
-                for (int i = 0; i < VL; i++) v[i] += x[i] * f;
-            }
-            if (whole) {
-                write_out<ELEM, VL>(a, sg, row, lane * VL, mm, ll, v, s_bad);
-            } else {
-                store_vec<VL>(slot + 2 * kRows + row * D + lane * VL, v);
-                if (lane == 0) *reinterpret_cast<float2*>(slot + 2 * row) = make_float2(mm, ll);
-            }
+                for (int j = 0; j < D / 16; j++)
+                    so[(nb * (D / 16) + j) * 32] =
+                        make_float4(o[j][nb][0], o[j][nb][1], o[j][nb][2], o[j][nb][3]);
         }
-        bool final = whole;
-        if (!whole) {
+        if (more) first_blocks(nx);
+        if (!final) {
             __threadfence();
-            __syncthreads();
-            if (threadIdx.x == 0) s_last = count_part(a, sg);
-            __syncthreads();
-            final = s_last;
+            __syncwarp();
+            int last = 0;
+            if (lane == 0) last = count_part(a, sg);
+            final = __shfl_sync(0xffffffffu, last, 0);
             if (final) {
                 __threadfence();
-                for (int row = warp; row < rows; row += kWarps) {
-                    float mm = -INFINITY, ll = 0.f, v[VL] = {};
-                    for (int p0 = 0; p0 < sg.parts; p0 += 32) {
-                        // lane i: maximum and sum of part p0 + i
-                        const int np = min(32, sg.parts - p0);
-                        float2 ml = make_float2(-INFINITY, 0.f);
-                        if (lane < np)
-                            ml = __ldcg(reinterpret_cast<const float2*>(
-                                part_slot(a, kRows, sg.first + p0 + lane, p0 + lane == 0) + 2 * row));
-                        float nm = ml.x;
-#pragma unroll
-                        for (int o2 = 16; o2 > 0; o2 >>= 1)
-                            nm = fmaxf(nm, __shfl_xor_sync(0xffffffffu, nm, o2));
-                        nm = fmaxf(nm, mm);
-                        const float b = nm == -INFINITY ? 0.f : nm;
-                        const float f = ex2(ml.x - b), back = ex2(mm - b);
-                        float sum = ml.y * f;
-#pragma unroll
-                        for (int o2 = 16; o2 > 0; o2 >>= 1)
-                            sum += __shfl_xor_sync(0xffffffffu, sum, o2);
-                        ll = ll * back + sum;
-#pragma unroll
-                        for (int i = 0; i < VL; i++) v[i] *= back;
-                        mm = nm;
-                        for (int p = 0; p < np; p += 8) {
-                            float x[8][VL];
-#pragma unroll
-                            for (int u = 0; u < 8; u++)
-                                if (p + u < np)
-                                    load_vec_cg<VL>(x[u], part_slot(a, kRows, sg.first + p0 + p + u,
-                                                                    p0 + p + u == 0) +
-                                                              2 * kRows + row * D + lane * VL);
-#pragma unroll
-                            for (int u = 0; u < 8; u++) {
-                                const float fu = __shfl_sync(0xffffffffu, f, (p + u) & 31);
-                                if (p + u < np) {
-#pragma unroll
-                                    for (int i = 0; i < VL; i++) v[i] = fmaf(x[u][i], fu, v[i]);
-                                }
-                            }
-                        }
-                    }
-                    write_out<ELEM, VL>(a, sg, row, lane * VL, mm, ll, v, s_bad);
-                }
+                join_parts<D, NB>(a, sg, o, m, l);
             }
         }
-        __syncthreads();
-        if (final) repair_rows(a, sg, rows, s_bad, warp, kWarps);
-        fence_async_smem();                          // the rings are TMA's again
-        __syncthreads();
+        if (final) finish_rows<D, ELEM, CT, NB>(a, sg, rows, o, m, l);
+        sg = nx;
+    }
+    if (!alive) {                                    // gave up: not before the copies have landed
+        volatile int never = 0;
+        for (; used != filled; used++)
+            mbar_wait_for(&s_full[warp][used % kStages], (used / kStages) & 1, &never, g_wait_limit_ns);
     }
 }
 
@@ -708,25 +710,19 @@ int row_blocks(const PagedAttn& a) {
     return (int)std::min<long long>((rows + 7) / 8, kMaxNB);
 }
 
-// How many pieces the work is cut into: those that start together, fewer when
-// the page table cannot hold that much work, and the small ones behind them.
-struct Pieces {
-    int blocks, extra;
-};
-int most_together(const PagedAttn& a) {
-    return std::min((row_blocks(a) == 1 ? 3 : 2) * num_sms(), kMaxBlocks / (1 + kExtra));
+// How many blocks share the work: all that fit the GPU, or fewer when the page
+// table cannot hold that much.
+int most_blocks(const PagedAttn& a) {
+    return std::min((row_blocks(a) == 1 ? 3 : 2) * num_sms(), kMaxPieces / kWarps);
 }
-Pieces pieces(const PagedAttn& a) {
-    const int nb = row_blocks(a), together = most_together(a);
-    const int step = kWarps * 4096 / (a.c.dim * (a.type >= kI8 ? 1 : 2));
+int blocks_for(const PagedAttn& a) {
+    const int step = 4096 / (a.c.dim * (a.type >= kI8 ? 1 : 2));
     const long long keys = (long long)a.tpages * a.c.ps;
-    const long long tile_tokens = 8 * nb / a.group;
+    const long long tile_tokens = 8 * row_blocks(a) / a.group;
     const long long tiles = (a.total_q + tile_tokens - 1) / tile_tokens + a.batch;
     const long long most = std::max(1LL, (keys + step - 1) / step) * std::min<long long>(tiles, 1 << 20) *
                            a.c.heads;
-    if (most <= (long long)together * 2 * kLeast)
-        return {(int)std::max(1LL, (most + kLeast - 1) / kLeast), 0};
-    return {together, kExtra * together};
+    return (int)std::min<long long>(most_blocks(a), (most + kLeast * kWarps - 1) / (kLeast * kWarps));
 }
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
@@ -783,13 +779,13 @@ int launch(const PagedAttn& a, cudaStream_t s) {
         if (e != cudaSuccess) return (int)e;
         attr_set.fetch_or(bit);
     }
-    const Pieces pc = pieces(a);
-    const SchedShape shape{C::ROWS / a.group, kWarps * C::BK, kLeast, pc.blocks, pc.extra, kShare};
+    const int blocks = blocks_for(a);
+    const SchedShape shape{C::ROWS / a.group, C::BK, kLeast, blocks * kWarps};
     int box = 8;                                     // tokens of a page side by side
     while (box < C::BK && a.c.ps % (2 * box) == 0) box *= 2;
     CUtensorMap tk, tv;
     if (!cache_map(&tk, a, a.c.k, C::RB, box) || !cache_map(&tv, a, a.c.v, C::RB, box)) return 1;
-    kern<<<pc.blocks + pc.extra, kThreads, C::SMEM, s>>>(tk, tv, a, shape, box);
+    kern<<<blocks, kThreads, C::SMEM, s>>>(tk, tv, a, shape, box);
     const cudaError_t e = cudaGetLastError();
     if (e == cudaSuccess) note_launch();
     return e == cudaSuccess ? 0 : (int)e;
@@ -816,7 +812,7 @@ int decode_max_rows() { return 8 * kMaxNB; }
 size_t paged_decode_workspace(const PagedAttn& a) {
     // (not by the length of the page table, which may grow between calls)
     return kCounterBytes +
-           2ull * (1 + kExtra) * most_together(a) * slot_floats(8 * row_blocks(a), a.c.dim) * sizeof(float);
+           2ull * kWarps * most_blocks(a) * slot_floats(8 * row_blocks(a), a.c.dim) * sizeof(float);
 }
 
 int paged_decode(const PagedAttn& a, cudaStream_t s) {

@@ -25,24 +25,7 @@ __device__ __forceinline__ float lse_of(float m2, float l) {
     return l == 0.f ? -INFINITY : m2 * 0.6931471805599453f + logf(l);
 }
 
-// columns d .. d + N - 1 of a row, v the unnormalised values, m2 and l the
-// row's maximum (log2 units) and sum
-template <int ELEM, int N>
-__device__ __forceinline__ void write_out(const PagedAttn& a, const Segment& g, int row, int d,
-                                          float m2, float l, const float (&v)[N], int* bad) {
-    const RowPlace r = row_place(a, g, row);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    char* o = a.o + (r.token * a.orow + r.head * a.oh + d) * 2;
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        const float x = v[i] * inv;
-        if (!isfinite(x)) bad[row] = 1;
-        store_as(o + 2 * i, ELEM, x);
-    }
-    if (d == 0 && a.lse) a.lse[r.head * a.lh + r.token] = lse_of(m2, l);
-}
-
-// by `warps` warps, after a barrier behind the last write_out
+// by a warp
 static __device__ __noinline__ void repair_row(const PagedAttn& a, const Segment& g, int row) {
     const RowPlace p = row_place(a, g, row);
     const int seen = keys_seen(a, g.q, p.token - g.q.q0);
@@ -51,10 +34,4 @@ static __device__ __noinline__ void repair_row(const PagedAttn& a, const Segment
     row_keys(a, g.s, a.q + (p.token * a.qr + p.head * a.qh) * 2, g.head, 0, seen, 32, r);
     row_store(a, p.token, p.head, r);
 }
-__device__ __forceinline__ void repair_rows(const PagedAttn& a, const Segment& g, int rows,
-                                            const int* bad, int warp, int warps) {
-    for (int row = warp; row < rows; row += warps)
-        if (bad[row]) repair_row(a, g, row);
-}
-
 }  // namespace zl

@@ -3,23 +3,22 @@
 // A unit is a tile of query rows of one sequence and KV head; its steps are
 // the key tiles that its rows see (one at least, so that rows which see
 // nothing are written too).  All steps of all units, in the order sequence,
-// head, tile, key, form one line, and block x takes the x-th piece of it:
-// `blocks` equal pieces that start together, and, where blocks of equal work
-// do not end together, `extra` small ones behind them that the hardware
-// starts wherever a block has ended.  Lengths live on the device, so every
-// block works its piece out from them: nothing is planned on the host, a
-// ragged batch is as even as a regular one, and a graph replays with new
-// lengths.  (Positions are 32 bits: 2^32 steps are minutes of work.)
+// head, tile, key, form one line, which is cut into equal pieces, one for
+// each worker (a block, or a warp where warps work alone).  Lengths live on
+// the device, so every worker finds its piece from them: nothing is planned
+// on the host, a ragged batch is as even as a regular one, and a graph
+// replays with new lengths.  (Positions are 32 bits: 2^32 steps are minutes
+// of work.)
 //
-// A unit that spans several blocks is joined by whichever of them finishes
+// A unit that spans several pieces is joined by whichever worker finishes
 // last: each leaves its unnormalised O with the maximum and the sum of every
 // row in the workspace and counts itself on the unit's counter; the last one
 // sums the parts in key order (so the result does not depend on who came
-// last) and puts the counter back to zero for the next call.  A block has at
-// most two partial units: one that began before its piece (slot 0, also
-// where it ends after it) and one that begins in it (slot 1).  The counter is
-// that of the block in which the unit begins, of which no other unit that
-// begins there runs out.
+// last) and puts the counter back to zero for the next call.  A piece has at
+// most two partial units: one that began before it (slot 0, also where it
+// ends after it) and one that begins in it (slot 1).  The counter is that of
+// the piece in which the unit begins, of which no other unit that begins
+// there runs out.
 #pragma once
 #include "paged.h"
 
@@ -29,18 +28,17 @@ struct SchedShape {
     int tokens;          // query tokens per tile
     int step;            // keys per step
     int least;           // steps per piece, at least
-    int blocks, extra;   // pieces of the first and of the second kind
-    int share;           // 256ths of the line that the first kind takes
+    int pieces;
 };
 
-// one block's piece of one unit
+// a unit, or what of it falls into one piece
 struct Segment {
     int s, head;         // sequence, KV head
     SeqInfo q;
     int i0, ni;          // the tile's first token in the chunk, and tokens
     int k0, k1;          // its keys in this piece (k1 is not rounded up)
-    int parts, part;     // blocks that share the unit; this block's place
-    int first;           // the block in which the unit begins
+    int parts, part;     // pieces that share the unit; this one's place
+    int first;           // the piece in which the unit begins
 };
 
 __device__ __forceinline__ int tile_end(const PagedAttn& a, const SeqInfo& q, int i1) {
@@ -75,11 +73,11 @@ __device__ __forceinline__ unsigned lane_sums(unsigned v) {
     return v;
 }
 
-// Walks a block's piece.  Every warp keeps one of its own (the search runs
+// Walks a piece.  Every warp keeps one of its own (the search runs
 // across the lanes; all lanes hold the same state afterwards).
 struct Walker {
     unsigned pos, end, begin;            // on the line; begin: of the unit
-    unsigned big, small, turn;           // piece sizes, and where the small ones start
+    unsigned per;                        // steps of a piece
     SeqInfo q;
     int s, head, tile;
     unsigned steps;
@@ -88,12 +86,7 @@ struct Walker {
         steps = tile_steps(a, h, q, tile);
     }
 
-    // the piece that holds a position
-    __device__ __forceinline__ unsigned piece_of(const SchedShape& h, unsigned p) const {
-        return p < turn ? p / big : h.blocks + (p - turn) / small;
-    }
-
-    __device__ void start(const PagedAttn& a, const SchedShape& h, int block) {
+    __device__ void start(const PagedAttn& a, const SchedShape& h, int piece) {
         const int lane = threadIdx.x & 31;
         // lane l sums sequences [l * each, (l + 1) * each)
         const int each = (a.batch + 31) / 32;
@@ -105,17 +98,9 @@ struct Walker {
         mine *= a.c.heads;
         const unsigned sum = lane_sums(mine);
         const unsigned total = __shfl_sync(0xffffffffu, sum, 31);
-        const unsigned fair = (total + h.blocks - 1) / h.blocks;
-        big = max((unsigned)h.least, h.extra ? (fair * h.share + 255) / 256 : fair);
-        turn = min(total, big * h.blocks);
-        small = h.extra ? max((unsigned)h.least, (total - turn + h.extra - 1) / h.extra) : 1;
-        if (block < h.blocks) {
-            pos = min(turn, block * big);
-            end = min(turn, pos + big);
-        } else {
-            pos = min(total, turn + (block - h.blocks) * small);
-            end = min(total, pos + small);
-        }
+        per = max((total + h.pieces - 1) / h.pieces, (unsigned)h.least);
+        pos = min((unsigned long long)total, (unsigned long long)piece * per);
+        end = min((unsigned long long)total, (unsigned long long)pos + per);
         if (pos >= end) return;
         // the lane whose sequences hold pos, then the sequence
         int l = __ffs(__ballot_sync(0xffffffffu, sum > pos)) - 1;
@@ -151,7 +136,7 @@ struct Walker {
     }
 
     // the next piece of a unit; false at the end of the line's piece
-    __device__ __forceinline__ bool next(const PagedAttn& a, const SchedShape& h, int block,
+    __device__ __forceinline__ bool next(const PagedAttn& a, const SchedShape& h, int piece,
                                          Segment& g) {
         if (pos >= end) return false;
         g.s = s;
@@ -167,11 +152,11 @@ struct Walker {
         if (st0 == 0 && st1 == steps) {
             g.parts = 1;
             g.part = 0;
-            g.first = block;
+            g.first = piece;
         } else {
-            g.first = (int)piece_of(h, begin);
-            g.parts = (int)piece_of(h, begin + steps - 1) - g.first + 1;
-            g.part = block - g.first;
+            g.first = (int)(begin / per);
+            g.parts = (int)((begin + steps - 1) / per) - g.first + 1;
+            g.part = piece - g.first;
         }
         pos = begin + st1;
         if (st1 == steps && pos < end) {
@@ -192,23 +177,21 @@ struct Walker {
 
 // ---- the workspace --------------------------------------------------------------
 
-constexpr int kMaxBlocks = 4096;                 // pieces; two counters each
-constexpr size_t kCounterBytes = 2 * kMaxBlocks * sizeof(int);
+constexpr int kMaxPieces = 2048;                 // two counters each
+constexpr size_t kCounterBytes = 2 * kMaxPieces * sizeof(int);
 
 // floats of one slot: (maximum, sum) of every row, then O
 __host__ __device__ constexpr long long slot_floats(int rows, int dim) {
     return (long long)rows * (2 + dim);
 }
 
-__device__ __forceinline__ float* part_slot(const PagedAttn& a, int rows, int block, bool begins) {
+__device__ __forceinline__ float* part_slot(const PagedAttn& a, int rows, int piece, bool begins) {
     return reinterpret_cast<float*>(a.ws + kCounterBytes) +
-           (2LL * block + (begins ? 1 : 0)) * slot_floats(rows, a.c.dim);
+           (2LL * piece + (begins ? 1 : 0)) * slot_floats(rows, a.c.dim);
 }
 
-// Called by every thread of a group of `threads` (a __syncthreads group or a
-// named barrier) after its part is stored and the group has synchronised
-// behind a __threadfence(): by one thread, which learns whether the part was
-// the unit's last.
+// Called by one thread of a worker once all its threads have stored their part
+// and passed a __threadfence() and a barrier: whether it was the unit's last.
 __device__ __forceinline__ bool count_part(const PagedAttn& a, const Segment& g) {
     int* counter = reinterpret_cast<int*>(a.ws) + g.first;
     const bool last = atomicAdd(counter, 1) == g.parts - 1;
