@@ -157,4 +157,6 @@ def test_python_checks(built_lib):
     with pytest.raises(ValueError):
         paged._type(torch.zeros(2, dtype=torch.float64))
     with pytest.raises(ValueError):
-        paged._index(torch.zeros(3, dtype=torch.int32), 1, "slots")
+        paged._index(torch.zeros(3, dtype=torch.int32), 0, "slots")
+    with pytest.raises(ValueError):
+        paged._table(torch.zeros(3, 4, dtype=torch.int32), 0)

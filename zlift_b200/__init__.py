@@ -126,7 +126,15 @@ def load(path: str | None = None) -> ctypes.CDLL:
 
 from .blas import Handle, GemmError  # noqa: E402
 from .attention import flash_forward, fmha_forward, FlashParams, FmhaParams  # noqa: E402
-from .paged import KVCache, kv_write, kv_read, paged_attention  # noqa: E402
+
+
+def __getattr__(name):
+    # the paged cache's calls need torch, which the rest of the package does not import
+    if name in ("KVCache", "kv_write", "kv_read", "paged_attention"):
+        from . import paged
+        return getattr(paged, name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
 
 __all__ = ["load", "Handle", "GemmError", "flash_forward", "fmha_forward",
            "FlashParams", "FmhaParams", "KVCache", "kv_write", "kv_read", "paged_attention",

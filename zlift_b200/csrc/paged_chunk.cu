@@ -24,14 +24,15 @@
 //           What a page holds behind the sequence's last token may be
 //           anything, NaN included, and 0 times that must be 0: those V rows
 //           are zeroed in shared memory before the tile is handed on.
-//   8 bit   Four warps load codes (16 bytes a lane, eight lanes a row of 128),
+//   8 bit   Three warps load codes (16 bytes a lane, eight lanes a row of 128),
 //           widen them to 16 bits exactly and store them in the swizzled
-//           layout that the tensor core reads.  The K scale of a key multiplies
+//           layout that the tensor core reads; K of the next tile is on its
+//           way while V of this one is widened, and the other way round.  The K scale of a key multiplies
 //           its column of S and the V scale its column of P, so nothing is
 //           rounded that a 16-bit cache would not round.
 //
 // Roles (warps): 0-3 and 4-7 softmax of tile 0 and 1, then the loaders (one
-// or four), then the MMA issuer.
+// or three), then the MMA issuer.
 #include "gemm.h"
 #include "paged_codes.cuh"
 #include "paged_finish.cuh"
@@ -52,7 +53,9 @@ template <int D, bool Q8>
 struct PCfg {
     static constexpr int BOXES = D / 64;
     static constexpr int TILE_BYTES = 128 * D * 2;
-    static constexpr int LOADERS = Q8 ? 4 : 1;               // warps
+    // warps; with three and the issuer a block has 12, the most that leave each
+    // thread 168 registers
+    static constexpr int LOADERS = Q8 ? 3 : 1;
     static constexpr int THREADS = 256 + LOADERS * 32 + 32;
     static constexpr int MMA_WARP = 8 + LOADERS;
     static constexpr int KV_OFF = 2 * TILE_BYTES;
@@ -82,8 +85,8 @@ struct Side {
     alignas(16) float vbig[kMaxBars][4];         // 8 bit: largest V scale of 32 keys
     alignas(16) float kscale[kMaxBars][BKEY];
     alignas(16) float vscale[kMaxBars][BKEY];
-    uint32_t rowat[2][BKEY];         // 8 bit: where a key's row is
-    Walker walk[13];
+    uint32_t rowat[3][BKEY];         // 8 bit: where a key's row is; three steps
+    Walker walk[12];
 };
 static_assert(sizeof(Side) <= 8192, "side area");
 
@@ -173,8 +176,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
         mbar_init(&sd.qempty, 1);
         mbar_init(&sd.vtail, 1);
         // 16 bit: the byte count's arrival, and "the tile is as it shall be";
-        // 8 bit: each of the four loader warps, once for K and once for V
-        for (int i = 0; i < KV_BARS; i++) mbar_init(&sd.kvfull[i], Q8 ? 8 : 2);
+        // 8 bit: each loader warp, once for K and once for V
+        for (int i = 0; i < KV_BARS; i++) mbar_init(&sd.kvfull[i], Q8 ? 2 * C::LOADERS : 2);
         for (int i = 0; i < NSLOT; i++) mbar_init(&sd.kvempty[i], 1);
         for (int i = 0; i < 2; i++) {
             mbar_init(&sd.sfull[i], 1);
@@ -204,7 +207,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
         bool ok = true;
         Segment sg;
         // (8 bit: a warp that gave up goes on through the named barriers that
-        // the other three may be waiting at)
+        // the others may be waiting at)
         while ((Q8 || ok) && next_segment(a, shape, &sd.walk[warp], sg)) {
             const Span sp = span_of(a, shape, sg);
             if (sp.nmax == 0) continue;
@@ -289,7 +292,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                 }
             } else {
                 constexpr int CPR = D / 16;          // 16-byte pieces of a row
-                constexpr int RP = 128 / CPR;        // rows per pass of the 128 threads
+                constexpr int LT = 32 * C::LOADERS;  // loader threads
+                constexpr int RP = LT / CPR;         // rows per pass of them
+                constexpr int NP = (BKEY + RP - 1) / RP;
                 constexpr uint32_t kNone = 0xffffffffu;
                 const int lt = threadIdx.x - 256, lw = warp - 8;
                 const int c = lt % CPR, r0 = lt / CPR;
@@ -297,86 +302,118 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                 const char* vb = a.c.v + sg.head * a.c.head + c * 16;
                 const float* ksb = a.c.ks + sg.head * a.c.shead;
                 const float* vsb = a.c.vs + sg.head * a.c.shead;
-                // thread lt looks up key lt of a tile
-                float ks = 0.f, vs = 0.f;
-                bool bad = false;
-                auto look_up = [&](int j, uint32_t buf) {
-                    const int key = (sp.s0 + j) * BKEY + lt;
-                    uint32_t at = kNone;
-                    ks = vs = 0.f;
-                    bad = false;
-                    if (j < sp.nmax && key < sg.q.len) {
-                        const unsigned i = a.c.by_ps.div(key);
-                        const int off = key - (int)i * a.c.ps;
-                        const int page = __ldg(table + i);
-                        if (page >= 0 && page < a.c.pages) {
-                            at = (uint32_t)((page * a.c.page + off * a.c.row) / 32);
-                            ks = __ldg(ksb + page * a.c.spage + off);
-                            vs = __ldg(vsb + page * a.c.spage + off);
-                        } else {
-                            bad = true;
-                            note_bad_index();
-                        }
-                    }
-                    sd.rowat[buf][lt] = at;
+                // Thread lt looks up key lt of a tile, and the first 32 the
+                // keys from 96 on: the row's place for all, its scales to keep.
+                struct Look {
+                    float ks[2], vs[2];
+                    bool bad[2];
                 };
-                named_bar_sync(3, 128);              // the last segment's rows are read
-                look_up(0, step & 1);
-                for (int j = 0; j < sp.nmax; j++, step++) {
-                    named_bar_sync(3, 128);
-                    uint4 w[2][CPR];
+                auto look_up = [&](int j, uint32_t buf) {
+                    Look q;
 #pragma unroll
-                    for (int i = 0; i < CPR; i++) {
-                        const uint32_t at = sd.rowat[step & 1][i * RP + r0];
-                        w[0][i] = w[1][i] = make_uint4(0u, 0u, 0u, 0u);
-                        if (at != kNone) {
-                            w[0][i] = __ldg(reinterpret_cast<const uint4*>(kb + (size_t)at * 32));
-                            w[1][i] = __ldg(reinterpret_cast<const uint4*>(vb + (size_t)at * 32));
+                    for (int h = 0; h < 2; h++) {
+                        const int i = h * LT + lt;
+                        const int key = (sp.s0 + j) * BKEY + i;
+                        uint32_t at = kNone;
+                        q.ks[h] = q.vs[h] = 0.f;
+                        q.bad[h] = false;
+                        if (i < BKEY && j < sp.nmax && key < sg.q.len) {
+                            const unsigned n = a.c.by_ps.div(key);
+                            const int off = key - (int)n * a.c.ps;
+                            const int page = __ldg(table + n);
+                            if (page >= 0 && page < a.c.pages) {
+                                at = (uint32_t)((page * a.c.page + off * a.c.row) / 32);
+                                q.ks[h] = __ldg(ksb + page * a.c.spage + off);
+                                q.vs[h] = __ldg(vsb + page * a.c.spage + off);
+                            } else {
+                                q.bad[h] = true;
+                                note_bad_index();
+                            }
+                        }
+                        if (i < BKEY) sd.rowat[buf][i] = at;
+                    }
+                    return q;
+                };
+                auto fetch = [&](uint4 (&w)[NP], const char* base, uint32_t buf) {
+#pragma unroll
+                    for (int i = 0; i < NP; i++) {
+                        const int row = i * RP + r0;
+                        const uint32_t at = row < BKEY ? sd.rowat[buf][row] : kNone;
+                        w[i] = make_uint4(0u, 0u, 0u, 0u);
+                        if (at != kNone) w[i] = __ldg(reinterpret_cast<const uint4*>(base + (size_t)at * 32));
+                    }
+                };
+                auto store = [&](const uint4 (&w)[NP], uint32_t slot) {
+                    uint8_t* dst = smem + C::KV_OFF + slot * C::TILE_BYTES + (c >> 2) * kBoxBytes;
+#pragma unroll
+                    for (int i = 0; i < NP; i++) {
+                        const int row = i * RP + r0;
+                        uint4 lo, hi;
+                        Code<ELEM, CT>::widen(w[i].x, lo.x, lo.y);
+                        Code<ELEM, CT>::widen(w[i].y, lo.z, lo.w);
+                        Code<ELEM, CT>::widen(w[i].z, hi.x, hi.y);
+                        Code<ELEM, CT>::widen(w[i].w, hi.z, hi.w);
+                        // 16-byte piece p of a row sits at p ^ (row % 8); the odd
+                        // half first where that spreads the eight lanes of a
+                        // row over all banks
+                        const int p = 2 * (c & 3), swap = c >> 2;
+                        uint8_t* d = dst + row * 128;
+                        if (row < BKEY) {
+                            *reinterpret_cast<uint4*>(d + ((p + swap) ^ (row & 7)) * 16) = swap ? hi : lo;
+                            *reinterpret_cast<uint4*>(d + ((p + 1 - swap) ^ (row & 7)) * 16) = swap ? lo : hi;
                         }
                     }
-                    const float ks_now = ks, vs_now = vs;
-                    const unsigned there = __ballot_sync(0xffffffffu, !bad);
-                    look_up(j + 1, (step + 1) & 1);
+                };
+                auto slot_free = [&](uint32_t item) {
+                    if (ok) ok = mbar_wait(&sd.kvempty[item % NSLOT], ((item / NSLOT) & 1) ^ 1u, abort_flag);
+                    ok = __all_sync(0xffffffffu, ok);
+                    return ok;
+                };
+                uint4 wk[NP], wv[NP];
+                uint32_t buf = 0;                    // of step j
+                auto after = [](uint32_t b, int n) { return (b + n) % 3; };
+                named_bar_sync(3, LT);               // the last segment's places are read
+                Look now = look_up(0, 0), next = look_up(1, 1);
+                named_bar_sync(3, LT);
+                fetch(wk, kb, 0);
+                fetch(wv, vb, 0);
+                for (int j = 0; j < sp.nmax; j++, step++, buf = after(buf, 1)) {
                     const int bar = step % KV_BARS;
+                    if (slot_free(2 * step)) {
 #pragma unroll
-                    for (int kv = 0; kv < 2; kv++) {
-                        const uint32_t item = 2 * step + kv, slot = item % NSLOT;
-                        if (ok) ok = mbar_wait(&sd.kvempty[slot], ((item / NSLOT) & 1) ^ 1u, abort_flag);
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) continue;           // (the named barrier still wants everyone)
-                        if (kv == 0) {
-                            sd.kscale[bar][lt] = ks_now;
-                            sd.vscale[bar][lt] = vs_now;
-                            float big = vs_now;
+                        for (int h = 0; h < 2; h++) {
+                            const int i = h * LT + lt;
+                            if (h == 1 && warp != 8) break;
+                            sd.kscale[bar][i] = now.ks[h];
+                            sd.vscale[bar][i] = now.vs[h];
+                            const unsigned there = __ballot_sync(0xffffffffu, !now.bad[h]);
+                            float big = now.vs[h];
 #pragma unroll
                             for (int o = 16; o > 0; o >>= 1)
                                 big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
                             if (lane == 0) {
-                                sd.there[bar][lw] = there;
-                                sd.vbig[bar][lw] = big;
+                                sd.there[bar][h ? 3 : lw] = there;
+                                sd.vbig[bar][h ? 3 : lw] = big;
                             }
                         }
-                        uint8_t* dst = smem + C::KV_OFF + slot * C::TILE_BYTES + (c >> 2) * kBoxBytes;
-#pragma unroll
-                        for (int i = 0; i < CPR; i++) {
-                            const int row = i * RP + r0;
-                            uint4 lo, hi;
-                            Code<ELEM, CT>::widen(w[kv][i].x, lo.x, lo.y);
-                            Code<ELEM, CT>::widen(w[kv][i].y, lo.z, lo.w);
-                            Code<ELEM, CT>::widen(w[kv][i].z, hi.x, hi.y);
-                            Code<ELEM, CT>::widen(w[kv][i].w, hi.z, hi.w);
-                            // 16-byte piece p of a row sits at p ^ (row % 8);
-                            // the odd half first where that spreads the eight
-                            // lanes of a row over all banks
-                            const int p = 2 * (c & 3), swap = c >> 2;
-                            uint8_t* d = dst + row * 128;
-                            *reinterpret_cast<uint4*>(d + ((p + swap) ^ (row & 7)) * 16) = swap ? hi : lo;
-                            *reinterpret_cast<uint4*>(d + ((p + 1 - swap) ^ (row & 7)) * 16) = swap ? lo : hi;
-                        }
+                        store(wk, (2 * step) % NSLOT);
                         fence_async_smem();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&sd.kvfull[bar]);
                     }
+                    // the places of step j + 1 were written a step ago, those of
+                    // j + 2 go where those of j - 1 were
+                    named_bar_sync(3, LT);
+                    fetch(wk, kb, after(buf, 1));
+                    now = next;
+                    next = look_up(j + 2, after(buf, 2));
+                    if (slot_free(2 * step + 1)) {
+                        store(wv, (2 * step + 1) % NSLOT);
+                        fence_async_smem();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sd.kvfull[bar]);
+                    }
+                    fetch(wv, vb, after(buf, 1));
                 }
             }
         }

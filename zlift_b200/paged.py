@@ -12,6 +12,9 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
+
+import torch
 
 from . import load
 
@@ -59,15 +62,19 @@ assert ctypes.sizeof(CacheBlock) == 96 and CacheBlock.num_pages.offset == 72
 assert ctypes.sizeof(RowsBlock) == 56 and RowsBlock.tokens.offset == 48
 assert ctypes.sizeof(AttnBlock) == 144 and AttnBlock.workspace.offset == 128
 
-_types = None
+# The structures are packed by hand in the calls below: filling a ctypes
+# Structure field by field costs several times as much.
+_rows_struct = struct.Struct("=2Q4q2i")
+_attn_struct = struct.Struct("=3Q5q3Qq7if2Q")
+assert _rows_struct.size == ctypes.sizeof(RowsBlock)
+assert _attn_struct.size == ctypes.sizeof(AttnBlock)
+
+_types = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32, torch.int8: I8,
+          torch.float8_e4m3fn: E4M3}
+_int32 = torch.int32
 
 
 def _type(t) -> int:
-    global _types
-    if _types is None:
-        import torch
-        _types = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32,
-                  torch.int8: I8, torch.float8_e4m3fn: E4M3}
     kind = _types.get(t.dtype)
     if kind is None:
         raise ValueError(f"no such element type: {t.dtype}")
@@ -79,12 +86,24 @@ def _need(ok, what):
         raise ValueError(what)
 
 
-def _index(t, dims, what):
-    import torch
-    _need(t.dtype == torch.int32 and t.dim() == dims and t.is_cuda and
-          (t.numel() < 2 or t.stride(-1) == 1),
-          f"{what}: an int32 CUDA tensor of {dims} dimension(s), contiguous along the last")
-    return t
+def _index(t, device, what):
+    """A one-dimensional index tensor on a device; returns its length."""
+    shape = t.shape
+    if t.dtype is not _int32 or len(shape) != 1 or t.get_device() != device or \
+            not t.is_contiguous():
+        raise ValueError(f"{what}: a contiguous int32 tensor of one dimension on the cache's GPU")
+    return shape[0]
+
+
+def _table(t, device):
+    """A page table; returns its shape and row stride."""
+    shape = t.shape
+    if t.dtype is not _int32 or len(shape) != 2 or t.get_device() != device:
+        raise ValueError("page_table: int32 [batch, pages] on the cache's GPU")
+    stride, one = t.stride()
+    if one != 1 and shape[1] > 1:
+        raise ValueError("page_table: a row's pages are contiguous")
+    return shape[0], shape[1], stride
 
 
 def _stream(stream) -> int:
@@ -100,7 +119,6 @@ class KVCache:
     """
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
-        import torch
         _need(k.dim() == 4 and k.shape == v.shape and k.stride() == v.stride() and
               k.dtype == v.dtype and k.is_cuda and k.device == v.device,
               "k and v: [pages, page_size, heads, dim] CUDA tensors of one type and layout")
@@ -124,62 +142,64 @@ class KVCache:
             b.k_scale, b.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
             b.scale_page_stride, b.scale_head_stride = k_scale.stride(0), k_scale.stride(1)
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.type, self.heads, self.dim, self.device = kind, b.heads, b.dim, k.device
+        self.type, self.heads, self.dim, self.device = kind, b.heads, b.dim, k.get_device()
+        self.softmax_scale = 1.0 / math.sqrt(b.dim)
         self.block = b
         self.ref = ctypes.byref(b)
 
     def _rows(self, k, v):
-        _need(k.dim() == 3 and k.shape == v.shape and k.shape[1] == self.heads and
-              k.shape[2] == self.dim and k.dtype == v.dtype and k.device == self.device and
-              v.device == self.device and k.stride(2) == v.stride(2) == 1,
-              "k and v: [tokens, heads, dim] of the cache's heads, dim and device")
-        r = RowsBlock()
-        r.k, r.v = k.data_ptr(), v.data_ptr()
-        r.k_row_stride, r.k_head_stride, _ = k.stride()
-        r.v_row_stride, r.v_head_stride, _ = v.stride()
-        r.tokens, r.elem = k.shape[0], _type(k)
-        return r
+        """zlift_kv_rows of packed k, v, and the number of tokens."""
+        shape, kind, device = k.shape, k.dtype, self.device
+        if len(shape) != 3 or shape != v.shape or shape[1] != self.heads or \
+                shape[2] != self.dim or v.dtype is not kind or k.get_device() != device or \
+                v.get_device() != device:
+            raise ValueError("k and v: [tokens, heads, dim] of one type, of the cache's heads, "
+                             "dim and GPU")
+        kr, kh, k1 = k.stride()
+        vr, vh, v1 = v.stride()
+        if (k1 != 1 or v1 != 1) and shape[2] > 1:
+            raise ValueError("k and v: dim is not contiguous")
+        return _rows_struct.pack(k.data_ptr(), v.data_ptr(), kr, kh, vr, vh, shape[0],
+                                 _type(k)), shape[0]
 
 
 def kv_write(cache: KVCache, k, v, slots, stream=None) -> int:
     """Writes packed k, v [tokens, heads, dim] into slots [tokens] (int32:
     page * page_size + offset; negative: skipped)."""
-    r = cache._rows(k, v)
-    _need(_index(slots, 1, "slots").shape[0] == r.tokens, "one slot for each token")
-    return load().zlift_kv_write(cache.ref, ctypes.byref(r), slots.data_ptr(), _stream(stream))
+    rows, tokens = cache._rows(k, v)
+    if _index(slots, cache.device, "slots") != tokens:
+        raise ValueError("one slot for each token")
+    return load().zlift_kv_write(cache.ref, rows, slots.data_ptr(),
+                                 0 if stream is None else _stream(stream))
 
 
 def kv_read(cache: KVCache, k_out, v_out, page_table, cu, starts=None, stream=None) -> int:
     """Reads tokens cu[s]..cu[s+1] of k_out, v_out [tokens, heads, dim] from
     positions starts[s] (default 0) onwards of sequence s, whose pages are
     page_table[s]."""
-    r = cache._rows(k_out, v_out)
-    _index(page_table, 2, "page_table")
-    batch = _index(cu, 1, "cu").shape[0] - 1
-    _need(batch >= 0 and page_table.shape[0] == batch, "cu has one entry more than page_table rows")
-    if starts is not None:
-        _need(_index(starts, 1, "starts").shape[0] == batch, "one start for each sequence")
-    return load().zlift_kv_read(cache.ref, ctypes.byref(r), page_table.data_ptr(),
-                                page_table.stride(0), page_table.shape[1],
+    rows, _ = cache._rows(k_out, v_out)
+    batch, pages, stride = _table(page_table, cache.device)
+    if _index(cu, cache.device, "cu") != batch + 1:
+        raise ValueError("cu has one entry more than page_table has rows")
+    if starts is not None and _index(starts, cache.device, "starts") != batch:
+        raise ValueError("one start for each sequence")
+    return load().zlift_kv_read(cache.ref, rows, page_table.data_ptr(), stride, pages,
                                 None if starts is None else starts.data_ptr(), cu.data_ptr(),
-                                batch, _stream(stream))
+                                batch, 0 if stream is None else _stream(stream))
 
 
 _workspaces = {}
 
 
-def _workspace(device, stream: int, nbytes: int):
+def _workspace(device: int, stream: int, nbytes: int):
     """The workspace of a device and stream: zeroed when made, replaced when a
     call wants more.  Made on that stream, so an older one is reused only
     after the work that still reads it."""
-    import torch
-    ws = _workspaces.get((device, stream))
-    if ws is None or ws.numel() < nbytes:
-        on = torch.cuda.ExternalStream(stream, device=device) if stream else \
-            torch.cuda.default_stream(device)
-        with torch.cuda.stream(on):
-            ws = torch.zeros(nbytes, dtype=torch.uint8, device=device)
-        _workspaces[(device, stream)] = ws
+    on = torch.cuda.ExternalStream(stream, device=device) if stream else \
+        torch.cuda.default_stream(device)
+    with torch.cuda.stream(on):
+        ws = torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", device))
+    _workspaces[(device, stream)] = ws
     return ws
 
 
@@ -194,46 +214,51 @@ def paged_attention(cache: KVCache, q, o, lse, page_table, cu_q, seq_k, max_q, c
     that no concurrent call uses; by default one per device and stream is
     kept (make one call outside a graph capture first, so that it exists).
     """
-    import torch
-    _need(q.dim() == 3 and q.shape == o.shape and q.dtype == o.dtype and
-          q.shape[2] == cache.dim and q.device == cache.device and o.device == cache.device and
-          q.stride(2) == o.stride(2) == 1, "q and o: [total_q, heads, dim] of one type")
-    _index(page_table, 2, "page_table")
-    batch = _index(seq_k, 1, "seq_k").shape[0]
-    _need(_index(cu_q, 1, "cu_q").shape[0] == batch + 1 and page_table.shape[0] == batch,
-          "cu_q has one entry more than seq_k and page_table rows")
-    p = AttnBlock()
-    p.q, p.o = q.data_ptr(), o.data_ptr()
-    p.q_row_stride, p.q_head_stride, _ = q.stride()
-    p.o_row_stride, p.o_head_stride, _ = o.stride()
+    device, kind, shape = cache.device, q.dtype, q.shape
+    if len(shape) != 3 or shape != o.shape or o.dtype is not kind or shape[2] != cache.dim or \
+            q.get_device() != device or o.get_device() != device:
+        raise ValueError("q and o: [total_q, heads, dim] of one type, of the cache's dim and GPU")
+    total, heads, _ = shape
+    qr, qh, q1 = q.stride()
+    orow, oh, o1 = o.stride()
+    if (q1 != 1 or o1 != 1) and shape[2] > 1:
+        raise ValueError("q and o: dim is not contiguous")
+    batch, pages, table_stride = _table(page_table, device)
+    if _index(seq_k, device, "seq_k") != batch or _index(cu_q, device, "cu_q") != batch + 1:
+        raise ValueError("seq_k has as many entries as page_table has rows, cu_q one more")
+    lse_ptr = lse_stride = 0
     if lse is not None:
-        _need(lse.dtype == torch.float32 and lse.shape == (q.shape[1], q.shape[0]) and
-              (lse.stride(1) == 1 or lse.shape[1] < 2) and lse.device == cache.device,
-              "lse: float32 [heads, total_q]")
-        p.lse, p.lse_head_stride = lse.data_ptr(), lse.stride(0)
-    p.cu_q, p.seq_k, p.page_table = cu_q.data_ptr(), seq_k.data_ptr(), page_table.data_ptr()
-    p.table_stride, p.table_pages = page_table.stride(0), page_table.shape[1]
-    p.batch, p.total_q, p.max_q, p.heads = batch, q.shape[0], int(max_q), q.shape[1]
-    p.elem, p.causal = _type(q), 1 if causal else 0
-    p.scale = 1.0 / math.sqrt(cache.dim) if scale is None else scale
-    lib, ref, s = load(), ctypes.byref(p), _stream(stream)
-    if workspace is None:
-        nbytes = lib.zlift_paged_attn_workspace(cache.ref, ref)
-        if nbytes:
-            workspace = _workspace(cache.device, s, nbytes)
-    if workspace is not None:
-        p.workspace, p.workspace_bytes = workspace.data_ptr(), workspace.numel()
-    return lib.zlift_paged_attn(cache.ref, ref, s)
+        lse_stride, l1 = lse.stride()
+        if lse.dtype is not torch.float32 or lse.shape != (heads, total) or \
+                (l1 != 1 and total > 1) or lse.get_device() != device:
+            raise ValueError("lse: float32 [heads, total_q], total_q contiguous")
+        lse_ptr = lse.data_ptr()
+    lib, s = load(), 0 if stream is None else _stream(stream)
+    ws = workspace if workspace is not None else _workspaces.get((device, s))
+    while True:
+        p = _attn_struct.pack(q.data_ptr(), o.data_ptr(), lse_ptr, qr, qh, orow, oh, lse_stride,
+                              cu_q.data_ptr(), seq_k.data_ptr(), page_table.data_ptr(),
+                              table_stride, pages, batch, total, int(max_q), heads, _type(q),
+                              1 if causal else 0, cache.softmax_scale if scale is None else scale,
+                              0 if ws is None else ws.data_ptr(),
+                              0 if ws is None else ws.numel())
+        rc = lib.zlift_paged_attn(cache.ref, p, s)
+        if rc != 1 or workspace is not None:
+            return rc
+        # declined: perhaps for want of (more) workspace
+        nbytes = lib.zlift_paged_attn_workspace(cache.ref, p)
+        if not nbytes or (ws is not None and ws.numel() >= nbytes):
+            return rc
+        ws = _workspace(device, s, nbytes)
 
 
 def attention_workspace(cache: KVCache, heads, total_q, max_q, batch, elem=None) -> int:
-    """Bytes of workspace that such calls of ``paged_attention`` want."""
-    p = AttnBlock()
-    p.batch, p.total_q, p.max_q, p.heads = batch, total_q, max_q, heads
-    p.elem = cache.type if cache.type < I8 else (BF16 if elem is None else elem)
-    p.scale = 1.0
+    """Bytes of workspace that such calls of ``paged_attention`` want (on
+    operands that the tensor cores can take)."""
+    if elem is None:
+        elem = cache.type if cache.type < I8 else BF16
     fake = 256                       # not followed: only sizes are looked at
-    p.q = p.o = p.cu_q = p.seq_k = p.page_table = fake
-    p.q_row_stride = p.o_row_stride = heads * cache.dim
-    p.q_head_stride = p.o_head_stride = cache.dim
-    return load().zlift_paged_attn_workspace(cache.ref, ctypes.byref(p))
+    row, head = heads * cache.dim, cache.dim
+    p = _attn_struct.pack(fake, fake, 0, row, head, row, head, 0, fake, fake, fake, 0, 0, batch,
+                          total_q, max_q, heads, elem, 1, 1.0, 0, 0)
+    return load().zlift_paged_attn_workspace(cache.ref, p)
