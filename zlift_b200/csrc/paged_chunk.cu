@@ -384,7 +384,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                         for (int h = 0; h < 2; h++) {
                             const int i = h * LT + lt;
                             if (h == 1 && warp != 8) break;
-                            sd.kscale[bar][i] = now.ks[h];
+                            sd.kscale[bar][i] = now.ks[h] * (a.scale * kLog2e);
                             sd.vscale[bar][i] = now.vs[h];
                             const unsigned there = __ballot_sync(0xffffffffu, !now.bad[h]);
                             float big = now.vs[h];
@@ -507,7 +507,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
         const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
         const uint32_t s_addr = tmem_base + lane_off + (t ? C::S_COL1 : C::S_COL0);
         const uint32_t o_addr = tmem_base + lane_off + (t ? C::O_COL1 : C::O_COL0);
-        const float c = a.scale * kLog2e;
+        const float c = Q8 ? 1.f : a.scale * kLog2e;     // 8 bit: in the K scales already
         // weights reach 2^lazy; in fp16 times a V scale of up to 512
         constexpr float kLazyLog2 = Q8 && ELEM == kF16 ? 6.f : 8.f;
         uint32_t step = 0, tiles = 0, finals = 0;
@@ -521,109 +521,211 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
             const bool row_ok = r < sg.ni * a.group;
             const int lim = row_ok ? tile_end(a, sg.q, sg.i0 + r / a.group + 1) : 0;
             const int lim_all = tile_end(a, sg.q, sg.i0 + 1);
-            float m_used = -INFINITY, l = 0.f;
-            float vmost = 0.f, vpow = 1.f, lpow = 0.f;
-            for (int j = 0; j < tnt && alive; j++, tiles++) {
-                alive = __all_sync(0xffffffffu, mbar_wait(&sd.sfull[t], tiles & 1, abort_flag));
-                if (!alive) break;
-                tc_fence_after();
-                const int bar = (step + j) % KV_BARS;
-                float s[BKEY];
+            float m_used = -INFINITY, l = 0.f, lpow = 0.f;
+            if constexpr (!Q8) {
+                for (int j = 0; j < tnt && alive; j++, tiles++) {
+                    alive = __all_sync(0xffffffffu, mbar_wait(&sd.sfull[t], tiles & 1, abort_flag));
+                    if (!alive) break;
+                    tc_fence_after();
+                    float s[BKEY];
 #pragma unroll
-                for (int c0 = 0; c0 < BKEY; c0 += 32)
-                    tmem_ld32(s_addr + c0, *reinterpret_cast<uint32_t(*)[32]>(&s[c0]));
-                tmem_wait_ld();
-                if constexpr (Q8) {
-                    const float4* ks = reinterpret_cast<const float4*>(sd.kscale[bar]);
+                    for (int c0 = 0; c0 < BKEY; c0 += 32)
+                        tmem_ld32(s_addr + c0, *reinterpret_cast<uint32_t(*)[32]>(&s[c0]));
+                    tmem_wait_ld();
+                    const int key0 = (sp.s0 + j) * BKEY;
+                    const uint4 th = *reinterpret_cast<const uint4*>(sd.there[(step + j) % KV_BARS]);
+                    if (key0 + BKEY > lim_all || (th.x & th.y & th.z & th.w) != 0xffffffffu) {
+                        const uint32_t tw[4] = {th.x, th.y, th.z, th.w};
 #pragma unroll
-                    for (int i = 0; i < BKEY / 4; i++) {
-                        const float4 f = ks[i];
-                        s[4 * i] *= f.x;
-                        s[4 * i + 1] *= f.y;
-                        s[4 * i + 2] *= f.z;
-                        s[4 * i + 3] *= f.w;
+                        for (int i = 0; i < BKEY; i++)
+                            if (key0 + i >= lim || !((tw[i >> 5] >> (i & 31)) & 1u)) s[i] = -INFINITY;
                     }
-                }
-                const int key0 = (sp.s0 + j) * BKEY;
-                const uint4 th = *reinterpret_cast<const uint4*>(sd.there[bar]);
-                const bool full = (th.x & th.y & th.z & th.w) == 0xffffffffu;
-                if (key0 + BKEY > lim_all || !full) {
-                    const uint32_t tw[4] = {th.x, th.y, th.z, th.w};
+                    float mx8[8];
 #pragma unroll
-                    for (int i = 0; i < BKEY; i++)
-                        if (key0 + i >= lim || !((tw[i >> 5] >> (i & 31)) & 1u)) s[i] = -INFINITY;
-                }
-                float mx8[8];
+                    for (int i = 0; i < 8; i++) mx8[i] = s[i];
 #pragma unroll
-                for (int i = 0; i < 8; i++) mx8[i] = s[i];
-#pragma unroll
-                for (int i = 8; i < BKEY; i++) mx8[i & 7] = fmaxf(mx8[i & 7], s[i]);
-                const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
-                                       fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
-                const float m_new = fmaxf(m_used, mx);
-                float vfix = 1.f;
-                if constexpr (Q8 && ELEM == kF16) {
-                    const float4 b = *reinterpret_cast<const float4*>(sd.vbig[bar]);
-                    vfix = v_power(fmaxf(fmaxf(b.x, b.y), fmaxf(b.z, b.w)), vmost, vpow);
-                    lpow = log2f(vpow);              // a power of two: exact
-                }
-                if (j == 0) {
-                    m_used = m_new;
-                } else {
-                    const bool grow = m_new != -INFINITY &&
-                                      (m_used == -INFINITY || (m_new - m_used) * c > kLazyLog2);
-                    if (__any_sync(0xffffffffu, grow || vfix != 1.f)) {
-                        float alpha = vfix;
-                        if (grow) {
-                            alpha *= ex2((m_used - m_new) * c);
-                            m_used = m_new;
-                        }
-                        l *= alpha;
+                    for (int i = 8; i < BKEY; i++) mx8[i & 7] = fmaxf(mx8[i & 7], s[i]);
+                    const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
+                                           fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
+                    const float m_new = fmaxf(m_used, mx);
+                    if (j == 0) {
+                        m_used = m_new;
+                    } else {
+                        const bool grow = m_new != -INFINITY &&
+                                          (m_used == -INFINITY || (m_new - m_used) * c > kLazyLog2);
+                        if (__any_sync(0xffffffffu, grow)) {
+                            float alpha = 1.f;
+                            if (grow) {
+                                alpha = ex2((m_used - m_new) * c);
+                                l *= alpha;
+                                m_used = m_new;
+                            }
 #pragma unroll 1
-                        for (int c0 = 0; c0 < D; c0 += 16) {
-                            uint32_t o[16];
-                            tmem_ld16(o_addr + c0, o);
-                            tmem_wait_ld();
+                            for (int c0 = 0; c0 < D; c0 += 16) {
+                                uint32_t o[16];
+                                tmem_ld16(o_addr + c0, o);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int i = 0; i < 16; i++)
+                                    o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                                tmem_st16(o_addr + c0, o);
+                            }
+                        }
+                    }
+                    const float mc = m_used == -INFINITY ? 0.f : m_used * c;
+                    float sum8[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int c0 = 0; c0 < BKEY / 2; c0 += 16) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const int k = 2 * (c0 + i);
+                            const float p0 = ex2(fmaf(s[k], c, -mc)), p1 = ex2(fmaf(s[k + 1], c, -mc));
+                            sum8[i & 7] += p0 + p1;
+                            pk[i] = pack2<ELEM>(p0, p1);
+                        }
+                        tmem_st16(s_addr + c0, pk);
+                    }
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) flag_add_release(&sd.pready[t]);
+                    l += ((sum8[0] + sum8[1]) + (sum8[2] + sum8[3])) +
+                         ((sum8[4] + sum8[5]) + (sum8[6] + sum8[7]));
+                }
+            } else {
+                // Every key has a factor of its own here.  With a whole row in a
+                // thread each thread would read all of them, and shared memory
+                // is what the tensor core lives on; as a matrix fragment,
+                // thread (g, t4) has 32 keys of the four rows g + 8k and reads the
+                // factors of those 32.
+                const int g = lane >> 2, t4 = lane & 3;
+                float m4[4], l4[4], b4[4];
+                int lim4[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    m4[k] = -INFINITY;
+                    l4[k] = b4[k] = 0.f;
+                    lim4[k] = __shfl_sync(0xffffffffu, lim, g + 8 * k);
+                }
+                float vmost = 0.f, vpow = 1.f;
+                for (int j = 0; j < tnt && alive; j++, tiles++) {
+                    alive = __all_sync(0xffffffffu, mbar_wait(&sd.sfull[t], tiles & 1, abort_flag));
+                    if (!alive) break;
+                    tc_fence_after();
+                    const int bar = (step + j) % KV_BARS;
+                    const float2* ks = reinterpret_cast<const float2*>(sd.kscale[bar]) + t4;
+                    const float2* vs = reinterpret_cast<const float2*>(sd.vscale[bar]) + t4;
+                    const int key0 = (sp.s0 + j) * BKEY;
+                    const uint4 th = *reinterpret_cast<const uint4*>(sd.there[bar]);
+                    const uint32_t tw[4] = {th.x, th.y, th.z, th.w};
+                    const bool edge = key0 + BKEY > lim_all ||
+                                      (th.x & th.y & th.z & th.w) != 0xffffffffu;
+                    float vfix = 1.f;
+                    if constexpr (ELEM == kF16) {
+                        const float4 b = *reinterpret_cast<const float4*>(sd.vbig[bar]);
+                        vfix = v_power(fmaxf(fmaxf(b.x, b.y), fmaxf(b.z, b.w)), vmost, vpow);
+                        if (vfix != 1.f) lpow = log2f(vpow);     // a power of two: exact
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {    // lanes 0-15, then 16-31
+                        const uint32_t half = (uint32_t)h << 20;
+                        float x[64];                 // scores in log2 units
+                        tmem_ld_frag128(s_addr + half, reinterpret_cast<uint32_t(&)[64]>(x));
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const float2 f = ks[4 * i];
+                            x[4 * i] *= f.x;
+                            x[4 * i + 1] *= f.y;
+                            x[4 * i + 2] *= f.x;
+                            x[4 * i + 3] *= f.y;
+                        }
+                        if (edge) {
 #pragma unroll
                             for (int i = 0; i < 16; i++)
-                                o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                            tmem_st16(o_addr + c0, o);
+#pragma unroll
+                                for (int e = 0; e < 2; e++) {
+                                    const int k = 8 * i + 2 * t4 + e;
+                                    const bool gone = !((tw[i >> 2] >> (k & 31)) & 1u);
+                                    if (gone || key0 + k >= lim4[2 * h]) x[4 * i + e] = -INFINITY;
+                                    if (gone || key0 + k >= lim4[2 * h + 1]) x[4 * i + 2 + e] = -INFINITY;
+                                }
                         }
+                        bool grow = vfix != 1.f;
+                        float alpha[2];
+#pragma unroll
+                        for (int r2 = 0; r2 < 2; r2++) {
+                            const int o = 2 * r2;
+                            float& mk = m4[2 * h + r2];
+                            float mx[4];
+#pragma unroll
+                            for (int i = 0; i < 4; i++) mx[i] = fmaxf(x[4 * i + o], x[4 * i + o + 1]);
+#pragma unroll
+                            for (int i = 4; i < 16; i++)
+                                mx[i & 3] = fmaxf(mx[i & 3], fmaxf(x[4 * i + o], x[4 * i + o + 1]));
+                            float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                            alpha[r2] = vfix;
+                            if (top > mk + kLazyLog2) {      // also from -inf
+                                alpha[r2] *= ex2(mk - top);
+                                mk = top;
+                                grow = true;
+                            }
+                        }
+                        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                            for (int r2 = 0; r2 < 2; r2++) {
+                                // the power of two rides in the exponent, on O and l alike
+                                b4[2 * h + r2] = (m4[2 * h + r2] == -INFINITY ? 0.f : m4[2 * h + r2]) - lpow;
+                                l4[2 * h + r2] *= alpha[r2];
+                            }
+                            if (j > 0) {
+#pragma unroll 1
+                                for (int c0 = 0; c0 < D; c0 += 32) {
+                                    uint32_t o[16];
+                                    tmem_ld_frag32(o_addr + half + c0, o);
+                                    tmem_wait_ld();
+#pragma unroll
+                                    for (int i = 0; i < 16; i++)
+                                        o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha[(i >> 1) & 1]);
+                                    tmem_st_frag32(o_addr + half + c0, o);
+                                }
+                            }
+                        }
+                        uint32_t pk[32];
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const float2 f = vs[4 * i];
+#pragma unroll
+                            for (int r2 = 0; r2 < 2; r2++) {
+                                const int o = 4 * i + 2 * r2;
+                                const float p0 = ex2(x[o] - b4[2 * h + r2]);
+                                const float p1 = ex2(x[o + 1] - b4[2 * h + r2]);
+                                l4[2 * h + r2] += p0 + p1;
+                                pk[2 * i + r2] = pack2<ELEM>(p0 * f.x, p1 * f.y);
+                            }
+                        }
+                        tmem_st_frag64(s_addr + half, pk);
+                    }
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) flag_add_release(&sd.pready[t]);
+                }
+                // back to a row for each thread: row `lane` of the warp's 32
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    l4[k] += __shfl_xor_sync(0xffffffffu, l4[k], 1);
+                    l4[k] += __shfl_xor_sync(0xffffffffu, l4[k], 2);
+                    const float mk = __shfl_sync(0xffffffffu, m4[k], (lane & 7) * 4);
+                    const float lk = __shfl_sync(0xffffffffu, l4[k], (lane & 7) * 4);
+                    if (k == lane >> 3) {
+                        m_used = mk;
+                        l = lk;
                     }
                 }
-                // the power of two rides in the exponent, on O and l alike
-                const float mc = (m_used == -INFINITY ? 0.f : m_used * c) - lpow;
-                float sum8[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                const float4* vsc = reinterpret_cast<const float4*>(sd.vscale[bar]);
-#pragma unroll
-                for (int c0 = 0; c0 < BKEY / 2; c0 += 16) {
-                    uint32_t pk[16];
-#pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        const int k = 2 * (c0 + i);
-                        float p[4];
-#pragma unroll
-                        for (int e = 0; e < 4; e++) p[e] = ex2(fmaf(s[k + e], c, -mc));
-                        sum8[i & 7] += p[0] + p[1];
-                        sum8[(i + 1) & 7] += p[2] + p[3];
-                        if constexpr (Q8) {
-                            const float4 f = vsc[k / 4];
-                            p[0] *= f.x;
-                            p[1] *= f.y;
-                            p[2] *= f.z;
-                            p[3] *= f.w;
-                        }
-                        pk[i] = pack2<ELEM>(p[0], p[1]);
-                        pk[i + 1] = pack2<ELEM>(p[2], p[3]);
-                    }
-                    tmem_st16(s_addr + c0, pk);
-                }
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) flag_add_release(&sd.pready[t]);
-                l += ((sum8[0] + sum8[1]) + (sum8[2] + sum8[3])) +
-                     ((sum8[4] + sum8[5]) + (sum8[6] + sum8[7]));
             }
             step += sp.nmax;
 
