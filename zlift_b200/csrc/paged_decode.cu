@@ -48,7 +48,8 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMaxNB = 3;
-constexpr int kLeast = 2;                // blocks of keys of a piece, at least
+constexpr int kMaxStages = 6;
+constexpr int kLeast = 3;                // blocks of keys of a piece, at least
 constexpr float kLazy = 6.f;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -66,11 +67,8 @@ struct DCfg {
     static constexpr int RB = D * EB > 128 ? 128 : D * EB;   // bytes of a row in a box
     static constexpr int CB = D * EB / RB;               // boxes side by side
     static constexpr int PER_SM = NB == 1 ? 3 : 2;       // blocks per SM
-    static constexpr int STAGES = NB == 1 ? 2 : 3;
-    static constexpr int RING = STAGES * 8192;
     static constexpr int SIDE = (Q8 ? 2 * BK * 4 : 0) + 16;  // scales, keys there; per stage
-    static constexpr int SIDE_OFF = kWarps * RING;
-    static constexpr int SMEM = SIDE_OFF + kWarps * STAGES * SIDE + 1024;
+    static constexpr int smem(int stages) { return kWarps * stages * (8192 + SIDE) + 1024; }
     static_assert(NT * KCH == 8 && BK / 4 * VCH * VP == 128, "a block is 8 KB");
 };
 
@@ -123,12 +121,9 @@ __device__ __forceinline__ void copy_async4(uint32_t dst, const float* src, bool
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;"
                  :: "r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
 }
-__device__ __forceinline__ void copy_commit() {
-    asm volatile("cp.async.commit_group;" ::: "memory");
-}
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-    asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory");
+// one arrival on `bar` once this thread's copies so far have landed
+__device__ __forceinline__ void copy_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(smem_u32(bar)) : "memory");
 }
 
 __device__ __forceinline__ uint4 lds16(uint32_t a) {
@@ -269,24 +264,25 @@ template <int D, int ELEM, int CT, int NB>
 __global__ void __launch_bounds__(kThreads, DCfg<D, CT, NB>::PER_SM)
 paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
                     const __grid_constant__ CUtensorMap tmV,
-                    const __grid_constant__ PagedAttn a, const SchedShape shape, const int box) {
+                    const __grid_constant__ PagedAttn a, const SchedShape shape, const int box,
+                    const uint32_t stages) {
     using C = DCfg<D, CT, NB>;
-    constexpr int kStages = C::STAGES;
     constexpr int MT = C::Q8 ? kF16 : ELEM;          // type of the products' operands
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    __shared__ uint64_t s_full[kWarps][kStages];
+    __shared__ uint64_t s_full[kWarps][kMaxStages];
     __shared__ int s_abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
     const int piece = blockIdx.x * kWarps + warp;
-    uint8_t* ring = smem + warp * C::RING;
-    const uint32_t side = smem_u32(smem + C::SIDE_OFF) + warp * kStages * C::SIDE;
+    uint8_t* ring = smem + warp * stages * 8192;
+    const uint32_t side = smem_u32(smem) + kWarps * stages * 8192 + warp * stages * C::SIDE;
     const float cscale = a.scale * kLog2e;
     if (threadIdx.x == 0) {
         for (int w = 0; w < kWarps; w++)
-            for (int i = 0; i < kStages; i++) mbar_init(&s_full[w][i], 1);
+            for (int i = 0; i < kMaxStages; i++)     // the bytes, and every lane's scales
+                mbar_init(&s_full[w][i], C::Q8 ? 33 : 1);
         s_abort = 0;
         fence_mbar_init();
     }
@@ -301,7 +297,16 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
     // the boxes this lane fetches: K or V, box column, box row
     const int box_kv = lane & 1, box_col = (lane >> 1) % C::CB, box_row = (lane >> 1) / C::CB;
     const bool box_mine = box_row * box < C::BK;
-    uint32_t filled = 0, used = 0;                   // blocks so far
+    struct Turn {                                    // a place in the ring, and its phase
+        uint32_t at = 0, phase = 0;
+        __device__ __forceinline__ void next(uint32_t n) {
+            if (++at == n) {
+                at = 0;
+                phase ^= 1;
+            }
+        }
+    } in, out;
+    int in_flight = 0;
     bool alive = true;
 
     Walker walk;
@@ -318,8 +323,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
                    ? __ldg(a.table + z.s * a.tstride + a.c.by_ps.div(key)) : -2;
     };
     auto load_block = [&](const Segment& z, int i, const int (&page)[PL]) {
-        const uint32_t stage = filled % kStages;
-        filled++;
+        const uint32_t stage = in.at;
+        in.next(stages);
+        in_flight++;
         uint32_t there[PL];
 #pragma unroll
         for (int h = 0; h < PL; h++) {
@@ -337,6 +343,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
                 }
             }
         }
+        if constexpr (C::Q8) copy_arrive(&s_full[warp][stage]);
         if (lane == 0) {
             asm volatile("st.shared.v2.u32 [%0], {%1,%2};" :: "r"(side + stage * C::SIDE),
                          "r"(there[0]), "r"(there[PL - 1]) : "memory");
@@ -360,20 +367,19 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
                         z.head, pg);
         }
     };
-    int page[kStages][PL];                           // of a segment's first blocks
+    // of a segment's first blocks, all but one of which are loaded ahead
+    int page[kMaxStages][PL];
     auto first_pages = [&](const Segment& z) {
 #pragma unroll
-        for (int i = 0; i < kStages; i++)
+        for (int i = 0; i < kMaxStages; i++)
 #pragma unroll
-            for (int h = 0; h < PL; h++) page[i][h] = page_at(z, i, h);
+            for (int h = 0; h < PL; h++) page[i][h] = i < stages ? page_at(z, i, h) : -2;
     };
     auto first_blocks = [&](const Segment& z) {
         const int n = blocks_of(z);
 #pragma unroll
-        for (int i = 0; i < kStages - 1; i++) {
-            if (i < n) load_block(z, i, page[i]);
-            copy_commit();
-        }
+        for (int i = 0; i < kMaxStages - 1; i++)
+            if (i < stages - 1 && i < n) load_block(z, i, page[i]);
     };
     if (more) {
         first_pages(sg);
@@ -385,7 +391,12 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
         const int mine = blocks_of(sg);
         int ahead[PL];                               // pages of the next block to load
 #pragma unroll
-        for (int h = 0; h < PL; h++) ahead[h] = page[kStages - 1][h];
+        for (int h = 0; h < PL; h++) {
+            ahead[h] = page[kMaxStages - 1][h];
+#pragma unroll
+            for (int i = 1; i < kMaxStages - 1; i++)
+                if (stages - 1 == i) ahead[h] = page[i][h];
+        }
 
         // ---- queries: row nb * 8 + g, dim permuted as the K pieces are
         uint32_t qb[D / 16][NB][2];
@@ -440,16 +451,15 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
 
         for (int i = 0; i < mine; i++) {
             __syncwarp();                            // the stage to fill is no longer read
-            if (i + kStages - 1 < mine) load_block(sg, i + kStages - 1, ahead);
+            if (i + (int)stages - 1 < mine) load_block(sg, i + stages - 1, ahead);
 #pragma unroll
-            for (int h = 0; h < PL; h++) ahead[h] = page_at(sg, i + kStages, h);
-            copy_commit();
-            const uint32_t stage = used % kStages;
+            for (int h = 0; h < PL; h++) ahead[h] = page_at(sg, i + stages, h);
+            const uint32_t stage = out.at;
             const uint32_t st = smem_u32(ring) + stage * 8192, sc = side + stage * C::SIDE;
-            copy_wait<kStages - 1>();
-            alive = __all_sync(0xffffffffu, mbar_wait(&s_full[warp][stage], (used / kStages) & 1, &s_abort));
+            alive = __all_sync(0xffffffffu, mbar_wait(&s_full[warp][stage], out.phase, &s_abort));
             if (!alive) break;
-            used++;
+            out.next(stages);
+            in_flight--;
             const int kb = sg.k0 + i * C::BK;
             // V rows past the keys, in a box that is partly wanted, may hold
             // anything: 0 times them must be 0
@@ -650,7 +660,6 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
                 }
             }
         }
-        copy_wait<0>();
 
         // ---- the next segment's pages are on their way while this one ends
         more = walk.next(a, shape, piece, nx);
@@ -699,8 +708,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
     }
     if (!alive) {                                    // gave up: not before the copies have landed
         volatile int never = 0;
-        for (; used != filled; used++)
-            mbar_wait_for(&s_full[warp][used % kStages], (used / kStages) & 1, &never, g_wait_limit_ns);
+        for (; in_flight > 0; in_flight--, out.next(stages))
+            mbar_wait_for(&s_full[warp][out.at], out.phase, &never, g_wait_limit_ns);
     }
 }
 
@@ -775,7 +784,8 @@ int launch(const PagedAttn& a, cudaStream_t s) {
     const unsigned long long bit = 1ull << (dev & 63);
     if (!(attr_set.load() & bit)) {
         const cudaError_t e =
-            cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+            cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 C::smem(kMaxStages));
         if (e != cudaSuccess) return (int)e;
         attr_set.fetch_or(bit);
     }
@@ -785,7 +795,11 @@ int launch(const PagedAttn& a, cudaStream_t s) {
     while (box < C::BK && a.c.ps % (2 * box) == 0) box *= 2;
     CUtensorMap tk, tv;
     if (!cache_map(&tk, a, a.c.k, C::RB, box) || !cache_map(&tv, a, a.c.v, C::RB, box)) return 1;
-    kern<<<blocks, kThreads, C::SMEM, s>>>(tk, tv, a, shape, box);
+    // stages that fit beside the other blocks of the SM; all of them where a
+    // block has its SM to itself
+    const int per_sm = (blocks + num_sms() - 1) / num_sms();
+    const int stages = per_sm == 1 ? kMaxStages : per_sm == 2 ? 3 : 2;
+    kern<<<blocks, kThreads, C::smem(stages), s>>>(tk, tv, a, shape, box, stages);
     const cudaError_t e = cudaGetLastError();
     if (e == cudaSuccess) note_launch();
     return e == cudaSuccess ? 0 : (int)e;
