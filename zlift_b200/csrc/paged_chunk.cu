@@ -24,7 +24,7 @@
 //           What a page holds behind the sequence's last token may be
 //           anything, NaN included, and 0 times that must be 0: those V rows
 //           are zeroed in shared memory before the tile is handed on.
-//   8 bit   Three warps load codes (16 bytes a lane, eight lanes a row of 128),
+//   8 bit   Six warps load codes (16 bytes a lane, eight lanes a row of 128),
 //           widen them to 16 bits exactly and store them in the swizzled
 //           layout that the tensor core reads; K of the next tile is on its
 //           way while V of this one is widened, and the other way round.  The K scale of a key multiplies
@@ -32,7 +32,7 @@
 //           rounded that a 16-bit cache would not round.
 //
 // Roles (warps): 0-3 and 4-7 softmax of tile 0 and 1, then the loaders (one
-// or three), then the MMA issuer.
+// or six), then the MMA issuer.
 #include "gemm.h"
 #include "paged_codes.cuh"
 #include "paged_finish.cuh"
@@ -53,9 +53,8 @@ template <int D, bool Q8>
 struct PCfg {
     static constexpr int BOXES = D / 64;
     static constexpr int TILE_BYTES = 128 * D * 2;
-    // warps; with three and the issuer a block has 12, the most that leave each
-    // thread 168 registers
-    static constexpr int LOADERS = Q8 ? 3 : 1;
+    // warps; with six and the issuer a block has 15, and 128 registers a thread
+    static constexpr int LOADERS = Q8 ? 6 : 1;
     static constexpr int THREADS = 256 + LOADERS * 32 + 32;
     static constexpr int MMA_WARP = 8 + LOADERS;
     static constexpr int KV_OFF = 2 * TILE_BYTES;
@@ -86,7 +85,7 @@ struct Side {
     alignas(16) float kscale[kMaxBars][BKEY];
     alignas(16) float vscale[kMaxBars][BKEY];
     uint32_t rowat[3][BKEY];         // 8 bit: where a key's row is; three steps
-    Walker walk[12];
+    Walker walk[15];
 };
 static_assert(sizeof(Side) <= 8192, "side area");
 
@@ -104,6 +103,30 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     } else {
         const __half2 v = __floats2half2_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&v);
+    }
+}
+
+// Piece c (16 codes) of rows r0, r0 + RP, ... widened to type T in a tile of
+// two (dim 64: one) swizzled column boxes.
+template <int T, int CT, int NP, int RP>
+__device__ __forceinline__ void store_codes(const uint4 (&w)[NP], uint8_t* tile, int c, int r0) {
+    uint8_t* dst = tile + (c >> 2) * kBoxBytes;
+    // 16-byte piece p of a row sits at p ^ (row % 8); the odd half first where
+    // that spreads the eight lanes of a row over all banks
+    const int p = 2 * (c & 3), swap = c >> 2;
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+        const int row = i * RP + r0;
+        uint4 lo, hi;
+        Code<T, CT>::widen(w[i].x, lo.x, lo.y);
+        Code<T, CT>::widen(w[i].y, lo.z, lo.w);
+        Code<T, CT>::widen(w[i].z, hi.x, hi.y);
+        Code<T, CT>::widen(w[i].w, hi.z, hi.w);
+        uint8_t* d = dst + row * 128;
+        if (row < BKEY) {
+            *reinterpret_cast<uint4*>(d + ((p + swap) ^ (row & 7)) * 16) = swap ? hi : lo;
+            *reinterpret_cast<uint4*>(d + ((p + 1 - swap) ^ (row & 7)) * 16) = swap ? lo : hi;
+        }
     }
 }
 
@@ -160,9 +183,12 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                    const __grid_constant__ PagedAttn a, const ChunkShape shape) {
     constexpr bool Q8 = CT >= kI8;
     using C = PCfg<D, Q8>;
+    // P and V of an 8-bit cache in fp16, to which codes widen most cheaply and
+    // in which weights keep three bits more than in bf16
+    constexpr int PV = Q8 ? kF16 : ELEM;
     constexpr int NSLOT = C::NSLOT, KV_BARS = C::KV_BARS;
     constexpr uint32_t IDESC_QK = make_idesc(1, ELEM == kBF16 ? 1 : 0, 0, 0, BQ, BKEY);
-    constexpr uint32_t IDESC_PV = make_idesc(1, ELEM == kBF16 ? 1 : 0, 0, 1, BQ, D);
+    constexpr uint32_t IDESC_PV = make_idesc(1, PV == kBF16 ? 1 : 0, 0, 1, BQ, D);
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -302,36 +328,30 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                 const char* vb = a.c.v + sg.head * a.c.head + c * 16;
                 const float* ksb = a.c.ks + sg.head * a.c.shead;
                 const float* vsb = a.c.vs + sg.head * a.c.shead;
-                // Thread lt looks up key lt of a tile, and the first 32 the
-                // keys from 96 on: the row's place for all, its scales to keep.
+                // Thread lt < 128 looks up key lt of a tile: the row's place for
+                // all, its scales to keep.
                 struct Look {
-                    float ks[2], vs[2];
-                    bool bad[2];
+                    float ks, vs;
+                    bool bad;
                 };
                 auto look_up = [&](int j, uint32_t buf) {
-                    Look q;
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const int i = h * LT + lt;
-                        const int key = (sp.s0 + j) * BKEY + i;
-                        uint32_t at = kNone;
-                        q.ks[h] = q.vs[h] = 0.f;
-                        q.bad[h] = false;
-                        if (i < BKEY && j < sp.nmax && key < sg.q.len) {
-                            const unsigned n = a.c.by_ps.div(key);
-                            const int off = key - (int)n * a.c.ps;
-                            const int page = __ldg(table + n);
-                            if (page >= 0 && page < a.c.pages) {
-                                at = (uint32_t)((page * a.c.page + off * a.c.row) / 32);
-                                q.ks[h] = __ldg(ksb + page * a.c.spage + off);
-                                q.vs[h] = __ldg(vsb + page * a.c.spage + off);
-                            } else {
-                                q.bad[h] = true;
-                                note_bad_index();
-                            }
+                    Look q{0.f, 0.f, false};
+                    const int key = (sp.s0 + j) * BKEY + lt;
+                    uint32_t at = kNone;
+                    if (lt < BKEY && j < sp.nmax && key < sg.q.len) {
+                        const unsigned n = a.c.by_ps.div(key);
+                        const int off = key - (int)n * a.c.ps;
+                        const int page = __ldg(table + n);
+                        if (page >= 0 && page < a.c.pages) {
+                            at = (uint32_t)((page * a.c.page + off * a.c.row) / 32);
+                            q.ks = __ldg(ksb + page * a.c.spage + off);
+                            q.vs = __ldg(vsb + page * a.c.spage + off);
+                        } else {
+                            q.bad = true;
+                            note_bad_index();
                         }
-                        if (i < BKEY) sd.rowat[buf][i] = at;
                     }
+                    if (lt < BKEY) sd.rowat[buf][lt] = at;
                     return q;
                 };
                 auto fetch = [&](uint4 (&w)[NP], const char* base, uint32_t buf) {
@@ -341,27 +361,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                         const uint32_t at = row < BKEY ? sd.rowat[buf][row] : kNone;
                         w[i] = make_uint4(0u, 0u, 0u, 0u);
                         if (at != kNone) w[i] = __ldg(reinterpret_cast<const uint4*>(base + (size_t)at * 32));
-                    }
-                };
-                auto store = [&](const uint4 (&w)[NP], uint32_t slot) {
-                    uint8_t* dst = smem + C::KV_OFF + slot * C::TILE_BYTES + (c >> 2) * kBoxBytes;
-#pragma unroll
-                    for (int i = 0; i < NP; i++) {
-                        const int row = i * RP + r0;
-                        uint4 lo, hi;
-                        Code<ELEM, CT>::widen(w[i].x, lo.x, lo.y);
-                        Code<ELEM, CT>::widen(w[i].y, lo.z, lo.w);
-                        Code<ELEM, CT>::widen(w[i].z, hi.x, hi.y);
-                        Code<ELEM, CT>::widen(w[i].w, hi.z, hi.w);
-                        // 16-byte piece p of a row sits at p ^ (row % 8); the odd
-                        // half first where that spreads the eight lanes of a
-                        // row over all banks
-                        const int p = 2 * (c & 3), swap = c >> 2;
-                        uint8_t* d = dst + row * 128;
-                        if (row < BKEY) {
-                            *reinterpret_cast<uint4*>(d + ((p + swap) ^ (row & 7)) * 16) = swap ? hi : lo;
-                            *reinterpret_cast<uint4*>(d + ((p + 1 - swap) ^ (row & 7)) * 16) = swap ? lo : hi;
-                        }
                     }
                 };
                 auto slot_free = [&](uint32_t item) {
@@ -380,23 +379,20 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                 for (int j = 0; j < sp.nmax; j++, step++, buf = after(buf, 1)) {
                     const int bar = step % KV_BARS;
                     if (slot_free(2 * step)) {
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const int i = h * LT + lt;
-                            if (h == 1 && warp != 8) break;
-                            sd.kscale[bar][i] = now.ks[h] * (a.scale * kLog2e);
-                            sd.vscale[bar][i] = now.vs[h];
-                            const unsigned there = __ballot_sync(0xffffffffu, !now.bad[h]);
-                            float big = now.vs[h];
+                        if (lw < BKEY / 32) {
+                            sd.kscale[bar][lt] = now.ks * (a.scale * kLog2e);
+                            sd.vscale[bar][lt] = now.vs;
+                            const unsigned there = __ballot_sync(0xffffffffu, !now.bad);
+                            float big = now.vs;
 #pragma unroll
                             for (int o = 16; o > 0; o >>= 1)
                                 big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
                             if (lane == 0) {
-                                sd.there[bar][h ? 3 : lw] = there;
-                                sd.vbig[bar][h ? 3 : lw] = big;
+                                sd.there[bar][lw] = there;
+                                sd.vbig[bar][lw] = big;
                             }
                         }
-                        store(wk, (2 * step) % NSLOT);
+                        store_codes<ELEM, CT, NP, RP>(wk, smem + C::KV_OFF + (2 * step) % NSLOT * C::TILE_BYTES, c, r0);
                         fence_async_smem();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&sd.kvfull[bar]);
@@ -408,7 +404,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                     now = next;
                     next = look_up(j + 2, after(buf, 2));
                     if (slot_free(2 * step + 1)) {
-                        store(wv, (2 * step + 1) % NSLOT);
+                        store_codes<PV, CT, NP, RP>(wv, smem + C::KV_OFF + (2 * step + 1) % NSLOT * C::TILE_BYTES, c, r0);
                         fence_async_smem();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&sd.kvfull[bar]);
@@ -509,7 +505,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
         const uint32_t o_addr = tmem_base + lane_off + (t ? C::O_COL1 : C::O_COL0);
         const float c = Q8 ? 1.f : a.scale * kLog2e;     // 8 bit: in the K scales already
         // weights reach 2^lazy; in fp16 times a V scale of up to 512
-        constexpr float kLazyLog2 = Q8 && ELEM == kF16 ? 6.f : 8.f;
+        constexpr float kLazyLog2 = Q8 ? 6.f : 8.f;
         uint32_t step = 0, tiles = 0, finals = 0;
         bool alive = true;
         Segment sg;
@@ -622,7 +618,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                     const bool edge = key0 + BKEY > lim_all ||
                                       (th.x & th.y & th.z & th.w) != 0xffffffffu;
                     float vfix = 1.f;
-                    if constexpr (ELEM == kF16) {
+                    {
                         const float4 b = *reinterpret_cast<const float4*>(sd.vbig[bar]);
                         vfix = v_power(fmaxf(fmaxf(b.x, b.y), fmaxf(b.z, b.w)), vmost, vpow);
                         if (vfix != 1.f) lpow = log2f(vpow);     // a power of two: exact
@@ -704,7 +700,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                                 const float p0 = ex2(x[o] - b4[2 * h + r2]);
                                 const float p1 = ex2(x[o + 1] - b4[2 * h + r2]);
                                 l4[2 * h + r2] += p0 + p1;
-                                pk[2 * i + r2] = pack2<ELEM>(p0 * f.x, p1 * f.y);
+                                pk[2 * i + r2] = pack2<PV>(p0 * f.x, p1 * f.y);
                             }
                         }
                         tmem_st_frag64(s_addr + half, pk);
