@@ -596,7 +596,12 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                 // thread (g, t4) has 32 keys of the four rows g + 8k and reads the
                 // factors of those 32.
                 const int g = lane >> 2, t4 = lane & 3;
-                float m4[4], l4[4], b4[4];
+                auto turn = [](auto& x, auto& y) {
+                    const auto z = x;
+                    x = y;
+                    y = z;
+                };
+                float m4[4], l4[4], b4[4];          // of rows g + 8k
                 int lim4[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
@@ -623,8 +628,12 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                         vfix = v_power(fmaxf(fmaxf(b.x, b.y), fmaxf(b.z, b.w)), vmost, vpow);
                         if (vfix != 1.f) lpow = log2f(vpow);     // a power of two: exact
                     }
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {    // lanes 0-15, then 16-31
+                    // Lanes 0-15, then 16-31, by one piece of code (unrolled
+                    // twice, it and the loaders' would not fit the instruction
+                    // cache together): the rows' state is turned round after
+                    // each.
+#pragma unroll 1
+                    for (int h = 0; h < 2; h++) {
                         const uint32_t half = (uint32_t)h << 20;
                         float x[64];                 // scores in log2 units
                         tmem_ld_frag128(s_addr + half, reinterpret_cast<uint32_t(&)[64]>(x));
@@ -644,8 +653,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                                 for (int e = 0; e < 2; e++) {
                                     const int k = 8 * i + 2 * t4 + e;
                                     const bool gone = !((tw[i >> 2] >> (k & 31)) & 1u);
-                                    if (gone || key0 + k >= lim4[2 * h]) x[4 * i + e] = -INFINITY;
-                                    if (gone || key0 + k >= lim4[2 * h + 1]) x[4 * i + 2 + e] = -INFINITY;
+                                    if (gone || key0 + k >= lim4[0]) x[4 * i + e] = -INFINITY;
+                                    if (gone || key0 + k >= lim4[1]) x[4 * i + 2 + e] = -INFINITY;
                                 }
                         }
                         bool grow = vfix != 1.f;
@@ -653,7 +662,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
 #pragma unroll
                         for (int r2 = 0; r2 < 2; r2++) {
                             const int o = 2 * r2;
-                            float& mk = m4[2 * h + r2];
+                            float& mk = m4[r2];
                             float mx[4];
 #pragma unroll
                             for (int i = 0; i < 4; i++) mx[i] = fmaxf(x[4 * i + o], x[4 * i + o + 1]);
@@ -674,8 +683,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
 #pragma unroll
                             for (int r2 = 0; r2 < 2; r2++) {
                                 // the power of two rides in the exponent, on O and l alike
-                                b4[2 * h + r2] = (m4[2 * h + r2] == -INFINITY ? 0.f : m4[2 * h + r2]) - lpow;
-                                l4[2 * h + r2] *= alpha[r2];
+                                b4[r2] = (m4[r2] == -INFINITY ? 0.f : m4[r2]) - lpow;
+                                l4[r2] *= alpha[r2];
                             }
                             if (j > 0) {
 #pragma unroll 1
@@ -690,20 +699,30 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                                 }
                             }
                         }
-                        uint32_t pk[32];
 #pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const float2 f = vs[4 * i];
+                        for (int i0 = 0; i0 < 16; i0 += 8) {
+                            uint32_t pk[16];
 #pragma unroll
-                            for (int r2 = 0; r2 < 2; r2++) {
-                                const int o = 4 * i + 2 * r2;
-                                const float p0 = ex2(x[o] - b4[2 * h + r2]);
-                                const float p1 = ex2(x[o + 1] - b4[2 * h + r2]);
-                                l4[2 * h + r2] += p0 + p1;
-                                pk[2 * i + r2] = pack2<PV>(p0 * f.x, p1 * f.y);
+                            for (int i = 0; i < 8; i++) {
+                                const float2 f = vs[4 * (i0 + i)];
+#pragma unroll
+                                for (int r2 = 0; r2 < 2; r2++) {
+                                    const int o = 4 * (i0 + i) + 2 * r2;
+                                    const float p0 = ex2(x[o] - b4[r2]);
+                                    const float p1 = ex2(x[o + 1] - b4[r2]);
+                                    l4[r2] += p0 + p1;
+                                    pk[2 * i + r2] = pack2<PV>(p0 * f.x, p1 * f.y);
+                                }
                             }
+                            tmem_st_frag32p(s_addr + half + 4 * i0, pk);
                         }
-                        tmem_st_frag64(s_addr + half, pk);
+#pragma unroll
+                        for (int k = 0; k < 2; k++) {
+                            turn(m4[k], m4[k + 2]);
+                            turn(l4[k], l4[k + 2]);
+                            turn(b4[k], b4[k + 2]);
+                            turn(lim4[k], lim4[k + 2]);
+                        }
                     }
                     tmem_wait_st();
                     tc_fence_before();
