@@ -175,6 +175,52 @@ __device__ __forceinline__ float* chunk_slot(const PagedAttn& a, int block, bool
            ((2LL * block + (begins ? 1 : 0)) * 2 + t) * slot_floats(BQ, D);
 }
 
+// Row r over the members of a join: maximum (log2 units) and sum, then 32
+// columns of O.
+template <int D>
+__device__ __forceinline__ void join_sums(const PagedAttn& a, const Segment& g, const Climb& c, int t,
+                                          int r, float& m2, float& l) {
+    float2 ml[kFan];
+    m2 = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kFan; u++) {
+        ml[u] = make_float2(-INFINITY, 0.f);
+        if (u < c.members)
+            ml[u] = __ldcg(reinterpret_cast<const float2*>(
+                chunk_slot<D>(a, g.first + c.part(u), c.part(u) == 0, t) + 2 * r));
+        m2 = fmaxf(m2, ml[u].x);
+    }
+    const float b = m2 == -INFINITY ? 0.f : m2;
+    l = 0.f;
+#pragma unroll
+    for (int u = 0; u < kFan; u++) l = fmaf(ml[u].y, ex2(ml[u].x - b), l);
+}
+template <int D>
+__device__ __forceinline__ void join_columns(const PagedAttn& a, const Segment& g, const Climb& c,
+                                             int t, int r, float m2, int c0, float (&v)[32]) {
+    const float b = m2 == -INFINITY ? 0.f : m2;
+#pragma unroll
+    for (int i = 0; i < 32; i++) v[i] = 0.f;
+#pragma unroll 1
+    for (int u = 0; u < c.members; u++) {
+        const float* ps = chunk_slot<D>(a, g.first + c.part(u), c.part(u) == 0, t);
+        const float pm = __ldcg(ps + 2 * r);
+        float4 x[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            x[i] = __ldcg(reinterpret_cast<const float4*>(ps + 2 * BQ + ((c0 / 4 + i) * BQ + r) * 4));
+        if (pm == -INFINITY) continue;               // its O may never have been written
+        const float f = ex2(pm - b);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            v[4 * i] = fmaf(x[i].x, f, v[4 * i]);
+            v[4 * i + 1] = fmaf(x[i].y, f, v[4 * i + 1]);
+            v[4 * i + 2] = fmaf(x[i].z, f, v[4 * i + 2]);
+            v[4 * i + 3] = fmaf(x[i].w, f, v[4 * i + 3]);
+        }
+    }
+}
+
 template <int D, int ELEM, int CT>
 __global__ void __launch_bounds__(PCfg<D, (CT >= kI8)>::THREADS, 1)
 paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
@@ -757,6 +803,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
             float m2 = m_used == -INFINITY ? -INFINITY : m_used * c - lpow;
             const bool split = sg.parts > 1;
             bool final = !split;
+            Climb up(sg);
             if (split) {
                 float* ps = chunk_slot<D>(a, blockIdx.x, sg.part == 0, t);
                 *reinterpret_cast<float2*>(ps + 2 * r) = make_float2(m2, l);
@@ -773,28 +820,34 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                                             __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
                     }
                 }
-                __threadfence();
-                named_bar_sync(1 + t, 128);
-                if (r == 0) {
-                    Segment u = sg;
-                    u.first = 2 * sg.first + t;      // a counter for each tile
-                    sd.last[t] = count_part(a, u);
-                }
-                named_bar_sync(1 + t, 128);
-                final = *static_cast<volatile int*>(&sd.last[t]);
-                named_bar_sync(1 + t, 128);          // (before the next segment writes it)
-                if (final) {
+#pragma unroll 1
+                for (;; up.up()) {
                     __threadfence();
-                    m2 = -INFINITY;
-                    for (int p = 0; p < sg.parts; p++)
-                        m2 = fmaxf(m2, __ldcg(chunk_slot<D>(a, sg.first + p, p == 0, t) + 2 * r));
-                    const float b = m2 == -INFINITY ? 0.f : m2;
-                    l = 0.f;
-                    for (int p = 0; p < sg.parts; p++) {
-                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(
-                            chunk_slot<D>(a, sg.first + p, p == 0, t) + 2 * r));
-                        l += ml.y * ex2(ml.x - b);
+                    named_bar_sync(1 + t, 128);
+                    if (r == 0) sd.last[t] = up.arrive(a, sg, t);
+                    named_bar_sync(1 + t, 128);
+                    const bool last = *static_cast<volatile int*>(&sd.last[t]);
+                    named_bar_sync(1 + t, 128);      // (before anyone writes it again)
+                    if (!last) break;
+                    __threadfence();
+                    join_sums<D>(a, sg, up, t, r, m2, l);
+                    if (up.top()) {
+                        final = true;
+                        break;
                     }
+                    if (up.members == 1) continue;
+                    // into the first member's slot, each thread its own row
+                    float* to = chunk_slot<D>(a, sg.first + up.part(0), up.part(0) == 0, t);
+#pragma unroll 1
+                    for (int c0 = 0; c0 < D; c0 += 32) {
+                        float v[32];
+                        join_columns<D>(a, sg, up, t, r, m2, c0, v);
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            *reinterpret_cast<float4*>(to + 2 * BQ + ((c0 / 4 + i) * BQ + r) * 4) =
+                                make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                    }
+                    *reinterpret_cast<float2*>(to + 2 * r) = make_float2(m2, l);
                 }
             }
             if (final && alive) {
@@ -814,24 +867,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                             for (int i = 0; i < 32; i++) v[i] = 0.f;
                         }
                     } else {
-#pragma unroll
-                        for (int i = 0; i < 32; i++) v[i] = 0.f;
-                        const float b = m2 == -INFINITY ? 0.f : m2;
-                        for (int p = 0; p < sg.parts; p++) {
-                            const float* ps = chunk_slot<D>(a, sg.first + p, p == 0, t);
-                            const float pm = __ldcg(ps + 2 * r);
-                            if (pm == -INFINITY) continue;       // its O was not written
-                            const float f = ex2(pm - b);
-#pragma unroll
-                            for (int i = 0; i < 8; i++) {
-                                const float4 x = __ldcg(reinterpret_cast<const float4*>(
-                                    ps + 2 * BQ + ((c0 / 4 + i) * BQ + r) * 4));
-                                v[4 * i] = fmaf(x.x, f, v[4 * i]);
-                                v[4 * i + 1] = fmaf(x.y, f, v[4 * i + 1]);
-                                v[4 * i + 2] = fmaf(x.z, f, v[4 * i + 2]);
-                                v[4 * i + 3] = fmaf(x.w, f, v[4 * i + 3]);
-                            }
-                        }
+                        join_columns<D>(a, sg, up, t, r, m2, c0, v);
                     }
                     if (row_ok) {
                         uint32_t w[16];

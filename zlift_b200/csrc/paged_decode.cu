@@ -169,20 +169,37 @@ __device__ __forceinline__ float halve_row(uint32_t (&qb)[D / 16][NB][2], int nb
     return __uint_as_float((uint32_t)(127 + e) << 23);
 }
 
-// Sums a unit's parts, in key order, into this warp's registers.
+// This warp's fragments to (and, summed in key order, from) part slots.
 template <int D, int NB>
-__device__ __forceinline__ void join_parts(const PagedAttn& a, const Segment& sg,
+__device__ __forceinline__ void store_part(float* slot, const float (&o)[D / 16][NB][4],
+                                           const float (&m)[NB][2], const float (&l)[NB][2]) {
+    const int lane = threadIdx.x & 31, t = lane & 3;
+    if (lane < 4) {
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+            reinterpret_cast<float4*>(slot)[nb * 4 + t] = make_float4(m[nb][0], l[nb][0], m[nb][1], l[nb][1]);
+    }
+    float4* so = reinterpret_cast<float4*>(slot + 16 * NB) + lane;
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+        for (int j = 0; j < D / 16; j++)
+            so[(nb * (D / 16) + j) * 32] = make_float4(o[j][nb][0], o[j][nb][1], o[j][nb][2], o[j][nb][3]);
+}
+
+template <int D, int NB>
+__device__ __forceinline__ void join_parts(const PagedAttn& a, const Segment& sg, const Climb& c,
                                            float (&o)[D / 16][NB][4], float (&m)[NB][2],
                                            float (&l)[NB][2]) {
     const int lane = threadIdx.x & 31, t = lane & 3;
-    auto slot = [&](int p) { return part_slot(a, 8 * NB, sg.first + p, p == 0); };
+    auto slot = [&](int u) { return part_slot(a, 8 * NB, sg.first + c.part(u), c.part(u) == 0); };
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
-        // maxima first (a load each, all independent), then sums, then O
+        // maxima first (a load each, all independent), then sums and O
         float mm[2] = {-INFINITY, -INFINITY};
-#pragma unroll 4
-        for (int p = 0; p < sg.parts; p++) {
-            const float4 ml = __ldcg(reinterpret_cast<const float4*>(slot(p)) + nb * 4 + t);
+#pragma unroll 8
+        for (int u = 0; u < c.members; u++) {
+            const float4 ml = __ldcg(reinterpret_cast<const float4*>(slot(u)) + nb * 4 + t);
             mm[0] = fmaxf(mm[0], ml.x);
             mm[1] = fmaxf(mm[1], ml.z);
         }
@@ -194,10 +211,10 @@ __device__ __forceinline__ void join_parts(const PagedAttn& a, const Segment& sg
         for (int j = 0; j < D / 16; j++)
 #pragma unroll
             for (int i = 0; i < 4; i++) o[j][nb][i] = 0.f;
-#pragma unroll 2
-        for (int p = 0; p < sg.parts; p++) {
-            const float4 ml = __ldcg(reinterpret_cast<const float4*>(slot(p)) + nb * 4 + t);
-            const float4* so = reinterpret_cast<const float4*>(slot(p) + 16 * NB) + lane;
+#pragma unroll 4
+        for (int u = 0; u < c.members; u++) {
+            const float4 ml = __ldcg(reinterpret_cast<const float4*>(slot(u)) + nb * 4 + t);
+            const float4* so = reinterpret_cast<const float4*>(slot(u) + 16 * NB) + lane;
             float4 v[D / 16];
 #pragma unroll
             for (int j = 0; j < D / 16; j++) v[j] = __ldcg(so + (nb * (D / 16) + j) * 32);
@@ -674,33 +691,27 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
                 m[nb][e] -= lpow;                    // log2 units, of O and l alike
             }
         bool final = sg.parts == 1;
-        if (!final) {
-            float* slot = part_slot(a, C::ROWS, piece, sg.part == 0);
-            if (g == 0) {
-#pragma unroll
-                for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-                    for (int e = 0; e < 2; e++)
-                        reinterpret_cast<float2*>(slot)[nb * 8 + 2 * t + e] = make_float2(m[nb][e], l[nb][e]);
-            }
-            float4* so = reinterpret_cast<float4*>(slot + 2 * C::ROWS) + lane;
-#pragma unroll
-            for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-                for (int j = 0; j < D / 16; j++)
-                    so[(nb * (D / 16) + j) * 32] =
-                        make_float4(o[j][nb][0], o[j][nb][1], o[j][nb][2], o[j][nb][3]);
-        }
+        if (!final) store_part<D, NB>(part_slot(a, C::ROWS, piece, sg.part == 0), o, m, l);
         if (more) first_blocks(nx);
         if (!final) {
-            __threadfence();
-            __syncwarp();
-            int last = 0;
-            if (lane == 0) last = count_part(a, sg);
-            final = __shfl_sync(0xffffffffu, last, 0);
-            if (final) {
+            Climb c(sg);
+#pragma unroll 1
+            for (;; c.up()) {
                 __threadfence();
-                join_parts<D, NB>(a, sg, o, m, l);
+                __syncwarp();
+                int last = 0;
+                if (lane == 0) last = c.arrive(a, sg, 0);
+                if (!__shfl_sync(0xffffffffu, last, 0)) break;
+                if (c.members > 1) {
+                    __threadfence();
+                    join_parts<D, NB>(a, sg, c, o, m, l);
+                }
+                if (c.top()) {
+                    final = true;
+                    break;
+                }
+                if (c.members > 1)
+                    store_part<D, NB>(part_slot(a, C::ROWS, sg.first + c.part(0), c.part(0) == 0), o, m, l);
             }
         }
         if (final) finish_rows<D, ELEM, CT, NB>(a, sg, rows, o, m, l);

@@ -12,13 +12,11 @@
 //
 // A unit that spans several pieces is joined by whichever worker finishes
 // last: each leaves its unnormalised O with the maximum and the sum of every
-// row in the workspace and counts itself on the unit's counter; the last one
-// sums the parts in key order (so the result does not depend on who came
-// last) and puts the counter back to zero for the next call.  A piece has at
-// most two partial units: one that began before it (slot 0, also where it
-// ends after it) and one that begins in it (slot 1).  The counter is that of
-// the piece in which the unit begins, of which no other unit that begins
-// there runs out.
+// row in the workspace and counts itself; the last one sums the parts in key
+// order (so the result does not depend on who came last) and puts the counter
+// back to zero for the next call.  A piece has at most two partial units: one
+// that began before it (slot 0, also where it ends after it) and one that
+// begins in it (slot 1).
 #pragma once
 #include "paged.h"
 
@@ -177,8 +175,10 @@ struct Walker {
 
 // ---- the workspace --------------------------------------------------------------
 
-constexpr int kMaxPieces = 2048;                 // two counters each
-constexpr size_t kCounterBytes = 2 * kMaxPieces * sizeof(int);
+constexpr int kMaxPieces = 2048;
+constexpr int kFan = 8;                          // parts joined at once
+constexpr int kLevels = 4;                       // kFan ^ kLevels >= kMaxPieces
+constexpr size_t kCounterBytes = kLevels * 2 * kMaxPieces * sizeof(int);
 
 // floats of one slot: (maximum, sum) of every row, then O
 __host__ __device__ constexpr long long slot_floats(int rows, int dim) {
@@ -190,13 +190,41 @@ __device__ __forceinline__ float* part_slot(const PagedAttn& a, int rows, int pi
            (2LL * piece + (begins ? 1 : 0)) * slot_floats(rows, a.c.dim);
 }
 
-// Called by one thread of a worker once all its threads have stored their part
-// and passed a __threadfence() and a barrier: whether it was the unit's last.
-__device__ __forceinline__ bool count_part(const PagedAttn& a, const Segment& g) {
-    int* counter = reinterpret_cast<int*>(a.ws) + g.first;
-    const bool last = atomicAdd(counter, 1) == g.parts - 1;
-    if (last) atomicExch(counter, 0);
-    return last;
-}
+// Joining many parts one after another would take longer than computing them,
+// so they are joined as a tree: parts 8i .. 8i + 7 by whichever of them comes
+// last, into the slot of part 8i; those sums the same way, and so on.  One
+// step of a worker's way up: what was part `index` of `count` (`stride` parts
+// each) belongs to `members` ones from `from` on.
+struct Climb {
+    int index, count, stride = 1, level = 0;
+    int from, members;
+    __device__ __forceinline__ Climb(const Segment& g) : index(g.part), count(g.parts) { look(); }
+    __device__ __forceinline__ void look() {
+        from = index / kFan * kFan;
+        members = min(kFan, count - from);
+    }
+    __device__ __forceinline__ bool top() const { return count <= kFan; }
+    __device__ __forceinline__ void up() {
+        index /= kFan;
+        count = (count + kFan - 1) / kFan;
+        stride *= kFan;
+        level++;
+        look();
+    }
+    // the part (of the unit's) whose slot holds member u
+    __device__ __forceinline__ int part(int u) const { return (from + u) * stride; }
+    // By one thread of a worker once all its threads have stored and passed a
+    // __threadfence() and a barrier: whether it was the last of the members.
+    // Counters are named by the piece of the first member; members of one unit
+    // are the only ones to share it where there are two or more.  `which` of two:
+    // the row tiles of a unit that joins them apart.
+    __device__ __forceinline__ bool arrive(const PagedAttn& a, const Segment& g, int which) const {
+        if (members == 1) return true;
+        int* counter = reinterpret_cast<int*>(a.ws) + level * 2 * kMaxPieces + 2 * (g.first + part(0)) + which;
+        const bool last = atomicAdd(counter, 1) == members - 1;
+        if (last) atomicExch(counter, 0);
+        return last;
+    }
+};
 
 }  // namespace zl
