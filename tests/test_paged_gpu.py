@@ -590,3 +590,68 @@ def test_small_workspace_is_declined_or_enough(cuda):
                                      workspace=ws[:need - 1]) == 1
         torch.cuda.synchronize()
         assert (o == 7).all()
+
+
+@pytest.mark.parametrize("held", ["int8", "fp8", "bf16"])
+def test_example_runs(cuda, held):
+    """examples/paged_serving.py: projections, cache and attention together,
+    against the contiguous forward on the same tokens."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples",
+                        "paged_serving.py")
+    spec = importlib.util.spec_from_file_location("paged_serving", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    mod.main(held)
+
+
+@pytest.mark.parametrize("held", ["same", "int8", "fp8"])
+@pytest.mark.parametrize("elem", ["bf16", "f16"])
+@pytest.mark.parametrize("new", [1, 70])
+def test_one_key_returns_its_value(cuda, elem, held, new):
+    """A query that sees one key gets that key's V: every code from the largest
+    to the subnormal ones, at any scale, within the two roundings (weight times
+    scale, and output) of each value itself."""
+    import torch
+    from zlift_b200 import paged
+    for size in (1e-3, 1.0, 30.0):
+        c = Case(elem, held, new=(new,), ctx=(new,), heads=4, kv_heads=2, dim=128, seed=int(size) + new)
+        v = c.v_in.float()
+        v[0] = size * torch.exp2(-torch.arange(128, device=cuda) / 6.0) * torch.sign(v[0])
+        c.v_in = v.to(c.v_in.dtype)
+        assert paged.kv_write(c.cache, c.k_in, c.v_in, c.slots) == 0
+        o, _ = c.run()
+        want = c.held64("v")[0].repeat_interleave(2, 0)
+        # (fp16 holds nothing below 2^-24)
+        bound = (2.01 * UNIT[elem]) * want.abs() + (2.0 ** -24 if elem == "f16" else 0.0)
+        assert ((o[0].double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("new,heads,kv_heads", [(1, 4, 1), (3, 8, 1), (33, 4, 1)])
+@pytest.mark.parametrize("held", ["same", "fp8"])
+def test_one_unit_over_the_whole_gpu(cuda, held, new, heads, kv_heads):
+    """One sequence and one KV head: every worker has a part of one unit."""
+    c = Case("bf16", held, new=(new,), ctx=(60000,), heads=heads, kv_heads=kv_heads, dim=128, page=64,
+             seed=new)
+    c.check()
+
+
+def test_calls_on_two_streams_keep_apart(cuda):
+    """Each stream has a workspace of its own."""
+    import torch
+    c = Case("bf16", "same", new=(1, 2), ctx=(3000, 500), heads=8, kv_heads=2, dim=128, seed=1)
+    d = Case("bf16", "int8", new=(40,), ctx=(2500,), heads=8, kv_heads=2, dim=128, seed=2)
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    c.run(stream=s1)
+    d.run(stream=s2)
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(10):
+        outs.append((c, c.run(stream=s1)))
+        outs.append((d, d.run(stream=s2)))
+    torch.cuda.synchronize()
+    for case, (o, lse) in outs:
+        eo, el, to, tl = case.exact()
+        assert ((o.double() - eo).abs() <= to).all() and ((lse.double() - el).abs() <= tl).all()
