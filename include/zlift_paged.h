@@ -21,8 +21,9 @@
  * Strides are in elements and may be anything (also negative or zero where
  * that makes sense for reading) unless stated; elements of one row (dim) are
  * contiguous.  The fast kernels need base pointers and strides that are
- * multiples of 16 bytes (attention: cache strides of 32) and dim 64 or 128;
- * everything else runs on the CUDA cores, correct and slower.
+ * multiples of 16 bytes (attention: cache strides of 32), dim 64 or 128,
+ * pages of a multiple of 8 tokens and a positive scale; everything else runs
+ * on the CUDA cores, correct and slower.
  */
 #ifndef ZLIFT_PAGED_H
 #define ZLIFT_PAGED_H
@@ -125,7 +126,8 @@ typedef struct zlift_paged_attn_params {
 /* Device bytes zlift_paged_attn wants for such a call (workspace fields not
  * read).  The workspace is 256-byte aligned and zero before its first use;
  * every call leaves it fit for the next one of any shape.  Calls that share
- * one must run one after another.  0 for calls that will be declined. */
+ * one must run one after another; after device error 1 (a wait ran out) it has
+ * to be zeroed again.  0 for calls that will be declined or need none. */
 ZLIFT_API size_t zlift_paged_attn_workspace(const zlift_kv_cache *cache,
                                             const zlift_paged_attn_params *p);
 

@@ -800,7 +800,7 @@ int zlift_set_wait_limit_ns(unsigned long long ns) {
     if (ns == 0) return CUBLAS_STATUS_INVALID_VALUE;
     const int r = gemm_tc_set_wait_limit(ns) | gemm_simt_set_wait_limit(ns) |
                   fmha_set_wait_limit(ns) | part_set_wait_limit(ns) |
-                  paged_chunk_set_wait_limit(ns);
+                  paged_decode_set_wait_limit(ns) | paged_chunk_set_wait_limit(ns);
     return r ? CUBLAS_STATUS_EXECUTION_FAILED : CUBLAS_STATUS_SUCCESS;
 }
 

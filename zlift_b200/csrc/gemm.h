@@ -137,6 +137,7 @@ int kv_cache_error(bool clear);
 int paged_simt_error(bool clear);
 int paged_decode_error(bool clear);
 int paged_chunk_error(bool clear);
+int paged_decode_set_wait_limit(unsigned long long ns);
 int paged_chunk_set_wait_limit(unsigned long long ns);
 
 // Trace switch (ZBLAS_TRACE set in the environment).

@@ -27,9 +27,18 @@
 //   8 bit   Six warps load codes (16 bytes a lane, eight lanes a row of 128),
 //           widen them to 16 bits exactly and store them in the swizzled
 //           layout that the tensor core reads; K of the next tile is on its
-//           way while V of this one is widened, and the other way round.  The K scale of a key multiplies
-//           its column of S and the V scale its column of P, so nothing is
-//           rounded that a 16-bit cache would not round.
+//           way while V of this one is widened, and the other way round.  The
+//           K scale of a key multiplies its column of S and the V scale its
+//           column of P, so nothing is rounded that a 16-bit cache would not
+//           round.
+//
+// Measured on one B200 (32/8 heads of 128): 512 new tokens over 32768, bf16,
+// 293 us in short runs (930 TFLOP/s), 344 us at the power cap; 4 ragged chunks
+// of up to 2048 over up to 4096 tokens, bf16 360 us, int8 565 us.  What 8 bits
+// cost there: instruction issue.  Three loader warps in place of six took 842
+// us; unrolling the softmax for both halves of a warp's rows 646 us, because
+// that code and the loaders' then overflow the instruction cache; a row of
+// scores per thread, whose 128 scales every thread reads, 760 us.
 //
 // Roles (warps): 0-3 and 4-7 softmax of tile 0 and 1, then the loaders (one
 // or six), then the MMA issuer.

@@ -2,38 +2,51 @@
 // paged cache: single tokens and short chunks, where reading the cache once
 // is the whole cost.
 //
-// Rows.  The group's query heads times the chunk's tokens are the rows of one
-// matrix operand (16 per tile), so K and V are read once for all of them.
-// Bytes bound it: per key and head 2 * dim * (2 or 1) bytes against 16 * dim
-// * 4 operations per 16 rows, some 64 operations a byte at most, far left of
-// the ridge.  That is why the products go through mma.sync m16n8k16 and not
-// tcgen05: operands come from registers in the layout that a plain row of the
-// cache already has, rows that do not exist cost little, and there is no
-// tile of 128 rows to fill nor a trip through tensor memory to wait for.
+// Bytes bound it: per key and KV head 2 * dim * (2 or 1) of them against 4 *
+// dim operations per row, and a row is a query head of the group times a
+// token: at most 24 rows here, so some 24 to 48 operations a byte, far left of
+// the ridge (250).  That is why the products go through mma.sync m16n8k16 and
+// not tcgen05: there is no tile of 128 rows to fill nor a trip through tensor
+// memory to wait for, and 8-bit codes become operands in registers.
 //
-// Loads.  A warp works alone: blocks of BK keys, its own online softmax, its
-// own ring of kStages blocks in shared memory filled by cp.async.  Each lane
-// fetches exactly the 16-byte pieces that it will itself use as operands, so
-// the ring needs no barrier, no swizzle and no bank conflicts (piece i of lane
-// l sits at i * 512 + l * 16).  The freedom that makes this work is the order
-// of the contraction: with the same permutation of dim on both sides,
-// q.k is unchanged, so lane (g, t) (g = lane / 4, t = lane % 4) takes 16
-// consecutive bytes of key g and the query operand is loaded to match; in P.V
-// it takes 16 consecutive bytes of its four keys, whose columns become the n
-// index of 8 or 16 products.  8-bit codes turn into 16-bit operands in
-// registers, exactly; a key's K scale multiplies its score and its V scale its
-// weight.
+// Products.  Keys are the long side: S^T = K.Q^T has 16 keys by 8 rows, O^T =
+// V^T.P^T 16 columns by 8 rows, so 8 rows (the usual group) waste nothing, and
+// NB = 1 to 3 blocks of 8 rows share every K and V operand.  P^T comes from S^T
+// by one 8 x 8 transposition in registers per 8 keys.  The contraction may
+// take dim in any order that both sides share: lane (g, t) = (lane / 4, lane %
+// 4) takes 16 consecutive bytes of key g, and the query operand is loaded to
+// match; in P.V it takes 16 consecutive bytes of its four keys, whose columns
+// become output rows g and g + 8 of the products.  Codes of an 8-bit cache widen
+// to fp16 exactly; a key's K scale multiplies its scores and its V scale its
+// weights.
+//
+// Loads.  A warp works alone on a piece of the keys (paged_sched.cuh): blocks
+// of 8 KB (16 to 64 keys, K and V), its own online softmax, its own ring of
+// blocks filled by TMA boxes of up to a page, in the swizzled layout in which
+// the lanes' 16-byte reads of V meet no bank conflict and those of K a double
+// one.  Lanes that copied their own operands by cp.async had fetched 1.6 times
+// the bytes from L2 (32-byte pieces of 64-byte requests): 172 against 124 us on
+// the case below.  The next segment's first blocks are asked for before this
+// one's rows are stored.
 //
 // Softmax in log2 units: x = s * scale * log2(e) (* K scale), weights
 // ex2(x - m) rounded to the 16-bit type for the product, summed unrounded in
 // fp32.  m is the running maximum, or up to 2^kLazy below it: O and l are
 // rescaled only when it grew by more, and both carry the same m, so the
-// quotient does not change.  In fp16 the V scale could leave the type's
-// range, so weights carry a power of two beside it that follows the largest V
-// scale seen.
+// quotient does not change.  In fp16 a V scale could leave the type's range:
+// see v_power.
 //
-// Work is split as in paged_sched.cuh; a block's four warps take blocks of
-// keys in turn and join through shared memory.
+// Measured on one B200 (32 query and 8 KV heads of 128 unless said otherwise):
+// 64 ragged sequences of up to 4096 bf16 tokens 124 us, 5.5 TB/s, 84% of the
+// copy rate; while all warps run it moves 6.4 TB/s, and the rest is that some
+// SMs get less of the memory than others and end 15% later.  Handing the last
+// 15 to 30% of the keys out in small pieces to whoever was free cost more in
+// parts to join than it gained (145 us and up).  16 x 32768 int8 176 us, 3.9
+// TB/s: per block of codes a warp issues some 600 instructions, half of them
+// widening, in one dependent chain.  32 sequences of up to 4096 e4m3 tokens with
+// 5 drafted ones 86 us (20 rows, three row blocks); 16 heads of 64, e4m3, 24 x
+// up to 2047 tokens 32 us; one bf16 sequence of 515 tokens, 8/2 heads 13 us,
+// all of it latency (launch, look-ups, first bytes, blocks, join).
 #include "gemm.h"
 #include "paged_codes.cuh"
 #include "paged_finish.cuh"
@@ -849,6 +862,8 @@ int paged_decode(const PagedAttn& a, cudaStream_t s) {
          : a.type == kE4M3 ? launch_dim<kF16, kE4M3>(a, s)
                            : launch_dim<kF16, kF16>(a, s);
 }
+
+int paged_decode_set_wait_limit(unsigned long long ns) { return set_unit_wait_limit(ns); }
 
 int paged_decode_error(bool clear) {
     int v = 0;
