@@ -375,7 +375,7 @@ bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Rows split into 8-element pieces whose lanes fit a warp, every piece
 // aligned: 16 bytes on a 16-bit side, 8 on an 8-bit one, 16 on an fp32 one.
-bool pieces(const KvView& c, int type, const Rows& r, int out_bytes) {
+bool pieces(const KvView& c, int type, const Rows& r) {
     if (c.dim != 32 && c.dim != 64 && c.dim != 128 && c.dim != 256) return false;
     const int eb = type >= kI8 ? 1 : 2;
     const long long m = type >= kI8 ? 8 : 16;
@@ -383,7 +383,6 @@ bool pieces(const KvView& c, int type, const Rows& r, int out_bytes) {
         if ((st * eb) % m) return false;
     for (long long st : {r.kr, r.kh, r.vr, r.vh})
         if (st % 16) return false;
-    (void)out_bytes;
     auto ok = [&](const void* p) { return (reinterpret_cast<uintptr_t>(p) & (m - 1)) == 0; };
     return ok(c.k) && ok(c.v) && al16(r.k) && al16(r.v);
 }
@@ -445,7 +444,7 @@ unsigned any_grid(const KvView& c, int tokens) {
 
 int kv_write(const KvView& c, int type, const zlift_kv_rows& z, const int* slots, cudaStream_t s) {
     const Rows r = make_rows(c, z);
-    if (!pieces(c, type, r, 2)) {
+    if (!pieces(c, type, r)) {
         kv_write_any_kernel<<<any_grid(c, r.tokens), kThreads, 0, s>>>(c, r, slots, z.elem, type);
         return done();
     }
@@ -463,7 +462,7 @@ int kv_read(const KvView& c, int type, const zlift_kv_rows& z, const int* table,
             cudaStream_t s) {
     const Rows r = make_rows(c, z);
     const Seqs q{table, starts, cu, tstride, tpages, batch};
-    if (!pieces(c, type, r, z.elem == kF32 ? 4 : 2)) {
+    if (!pieces(c, type, r)) {
         kv_read_any_kernel<<<any_grid(c, r.tokens), kThreads, 0, s>>>(c, r, q, type, z.elem);
         return done();
     }
