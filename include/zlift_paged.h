@@ -16,7 +16,8 @@
  * outside the cache is never followed.  A write to it is dropped, a read of
  * it gives zeros, attention treats its keys as absent, and
  * zlift_device_error() then reports 2.  Lengths are clamped to what the page
- * table and `total_q` can hold.
+ * table and `total_q` can hold.  Index arrays must not change while a call
+ * that reads them runs.
  *
  * Strides are in elements and may be anything (also negative or zero where
  * that makes sense for reading) unless stated; elements of one row (dim) are

@@ -164,8 +164,11 @@ class Case:
     def run(self, causal=True, scale=None, max_q=None, stream=None, o=None, lse=True, q=None, **kw):
         import torch
         from zlift_b200 import paged
-        o = torch.full_like(self.q, 7.0) if o is None else o
+        made = o is None
+        o = torch.full_like(self.q, 7.0) if made else o
         ls = torch.full((self.heads, self.total_q), 7.0, device=self.dev) if lse is True else lse
+        if made and stream is not None:                      # filled on this stream, used on that
+            torch.cuda.current_stream().synchronize()
         rc = paged.paged_attention(self.cache, self.q if q is None else q, o, ls, self.table, self.cu,
                                    self.lens, max(self.new) if max_q is None else max_q,
                                    causal=causal, scale=scale, stream=stream, **kw)
@@ -655,3 +658,21 @@ def test_calls_on_two_streams_keep_apart(cuda):
     for case, (o, lse) in outs:
         eo, el, to, tl = case.exact()
         assert ((o.double() - eo).abs() <= to).all() and ((lse.double() - el).abs() <= tl).all()
+
+
+def test_a_capture_makes_no_workspace(cuda):
+    """A stream without a workspace says so under capture, where memory would
+    be the graph's."""
+    import torch
+    c = Case("bf16", "same", new=(1,), ctx=(300,), heads=8, kv_heads=2, dim=128)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    from zlift_b200 import paged
+    paged._workspaces.pop((c.cache.device, s.cuda_stream), None)
+    o, lse = torch.full_like(c.q, 7.0), torch.empty(8, 1, device=cuda)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=s):
+        with pytest.raises(RuntimeError):
+            c.run(stream=s, o=o, lse=lse)
+    torch.cuda.synchronize()
+    c.check(stream=s)

@@ -105,7 +105,7 @@ struct Walker {
         unsigned base = __shfl_sync(0xffffffffu, sum - mine, l);
         s = l * each;
         if (each > 1) {
-            for (int b0 = l * each;; b0 += 32) {
+            for (int b0 = l * each; b0 < (l + 1) * each; b0 += 32) {
                 const int b = b0 + lane;
                 const unsigned v = b < min(a.batch, (l + 1) * each)
                                        ? head_steps(a, h, seq_info(a, b)) * a.c.heads : 0;
@@ -121,12 +121,12 @@ struct Walker {
             }
         }
         q = seq_info(a, s);
-        const unsigned hs = head_steps(a, h, q);
-        head = (int)((pos - base) / hs);
+        const unsigned hs = max(1u, head_steps(a, h, q));
+        head = min((int)((pos - base) / hs), a.c.heads - 1);
         begin = base + head * hs;
         tile = 0;
         enter(a, h);
-        while (pos - begin >= steps) {
+        while (pos - begin >= steps && (tile + 1) * h.tokens < q.n) {
             begin += steps;
             tile++;
             enter(a, h);
@@ -164,7 +164,7 @@ struct Walker {
                 if (++head == a.c.heads) {
                     head = 0;
                     do q = seq_info(a, ++s);
-                    while (q.n == 0);
+                    while (q.n == 0 && s + 1 < a.batch);
                 }
             }
             enter(a, h);

@@ -198,6 +198,9 @@ def _workspace(device: int, stream: int, nbytes: int):
     on = torch.cuda.ExternalStream(stream, device=device) if stream else \
         torch.cuda.default_stream(device)
     with torch.cuda.stream(on):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("no workspace for this stream yet: call once before the capture, "
+                               "or pass workspace=")
         ws = torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", device))
     _workspaces[(device, stream)] = ws
     return ws
