@@ -110,7 +110,7 @@ Way choose(const PagedAttn& a) {
                        (a.orow * 2) % 16 == 0 && (a.oh * 2) % 16 == 0;
     // Few rows go to the kernel that reads the cache once for 24 of them; more,
     // to the one with tiles of 128 rows.  20 rows (5 tokens, group 4, 32 x up to
-    // 4096 e4m3 tokens) took 86 us in the first and 320 us in the second.
+    // 4096 e4m3 tokens) took 80 us in the first and 320 us in the second.
     const long long rows = (long long)(a.max_q > 1 ? a.max_q : 1) * a.group;
     if (a.group <= decode_max_rows() && (rows <= decode_max_rows() || !boxes)) return Way::Decode;
     return boxes ? Way::Chunk : Way::Simt;

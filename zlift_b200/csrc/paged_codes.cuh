@@ -40,14 +40,15 @@ struct Code<kBF16, kI8> {
     }
 };
 
-// e4m3 -> fp16 by the hardware's conversion of two codes (exact)
+// e4m3 -> fp16 by the hardware's conversion of two codes (exact; two
+// instructions a word, where taking the halves apart in C++ cost more: drafted
+// tokens 86 against 80 us)
 template <>
 struct Code<kF16, kE4M3> {
     static __device__ __forceinline__ void widen(uint32_t u, uint32_t& lo, uint32_t& hi) {
-        const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(u & 0xffffu), __NV_E4M3);
-        const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(u >> 16), __NV_E4M3);
-        lo = (uint32_t)a.x | (uint32_t)a.y << 16;
-        hi = (uint32_t)b.x | (uint32_t)b.y << 16;
+        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+            "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+            : "=r"(lo), "=r"(hi) : "r"(u));
     }
 };
 

@@ -44,8 +44,8 @@
 // parts to join than it gained (145 us and up).  16 x 32768 int8 176 us, 3.9
 // TB/s: per block of codes a warp issues some 600 instructions, half of them
 // widening, in one dependent chain.  32 sequences of up to 4096 e4m3 tokens with
-// 5 drafted ones 86 us (20 rows, three row blocks); 16 heads of 64, e4m3, 24 x
-// up to 2047 tokens 32 us; one bf16 sequence of 515 tokens, 8/2 heads 13 us,
+// 5 drafted ones 80 us (20 rows, three row blocks); 16 heads of 64, e4m3, 24 x
+// up to 2047 tokens 29 us; one bf16 sequence of 515 tokens, 8/2 heads 13 us,
 // all of it latency (launch, look-ups, first bytes, blocks, join).
 #include "gemm.h"
 #include "paged_codes.cuh"
