@@ -90,7 +90,8 @@ struct Side {
     int abort;
     int last[2];
     alignas(16) uint32_t there[kMaxBars][4];     // which keys of the tile are in the cache
-    alignas(16) float vbig[kMaxBars][4];         // 8 bit: largest V scale of 32 keys
+    alignas(16) uint32_t vbig[kMaxBars][4];      // 8 bit: largest V scale of 32 keys,
+    alignas(16) uint32_t vleast[kMaxBars][4];    // and the smallest (scale_key)
     alignas(16) float kscale[kMaxBars][BKEY];
     alignas(16) float vscale[kMaxBars][BKEY];
     uint32_t rowat[3][BKEY];         // 8 bit: where a key's row is; three steps
@@ -197,7 +198,7 @@ __device__ __forceinline__ void join_sums(const PagedAttn& a, const Segment& g, 
         if (u < c.members)
             ml[u] = __ldcg(reinterpret_cast<const float2*>(
                 chunk_slot<D>(a, g.first + c.part(u), c.part(u) == 0, t) + 2 * r));
-        m2 = fmaxf(m2, ml[u].x);
+        m2 = max_nan(m2, ml[u].x);
     }
     const float b = m2 == -INFINITY ? 0.f : m2;
     l = 0.f;
@@ -438,13 +439,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                             sd.kscale[bar][lt] = now.ks * (a.scale * kLog2e);
                             sd.vscale[bar][lt] = now.vs;
                             const unsigned there = __ballot_sync(0xffffffffu, !now.bad);
-                            float big = now.vs;
-#pragma unroll
-                            for (int o = 16; o > 0; o >>= 1)
-                                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+                            const uint32_t big = __reduce_max_sync(0xffffffffu, scale_key(now.vs, 0u));
+                            const uint32_t least =
+                                __reduce_min_sync(0xffffffffu, scale_key(now.vs, 0xffffffffu));
                             if (lane == 0) {
                                 sd.there[bar][lw] = there;
                                 sd.vbig[bar][lw] = big;
+                                sd.vleast[bar][lw] = least;
                             }
                         }
                         store_codes<ELEM, CT, NP, RP>(wk, smem + C::KV_OFF + (2 * step) % NSLOT * C::TILE_BYTES, c, r0);
@@ -573,6 +574,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
             const int lim = row_ok ? tile_end(a, sg.q, sg.i0 + r / a.group + 1) : 0;
             const int lim_all = tile_end(a, sg.q, sg.i0 + 1);
             float m_used = -INFINITY, l = 0.f, lpow = 0.f;
+            float vmost = 0.f, vpow = 1.f;           // 8 bit: see v_power
+            uint32_t vleast = 0xffffffffu;
             if constexpr (!Q8) {
                 for (int j = 0; j < tnt && alive; j++, tiles++) {
                     alive = __all_sync(0xffffffffu, mbar_wait(&sd.sfull[t], tiles & 1, abort_flag));
@@ -664,7 +667,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                     l4[k] = b4[k] = 0.f;
                     lim4[k] = __shfl_sync(0xffffffffu, lim, g + 8 * k);
                 }
-                float vmost = 0.f, vpow = 1.f;
                 for (int j = 0; j < tnt && alive; j++, tiles++) {
                     alive = __all_sync(0xffffffffu, mbar_wait(&sd.sfull[t], tiles & 1, abort_flag));
                     if (!alive) break;
@@ -679,9 +681,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                                       (th.x & th.y & th.z & th.w) != 0xffffffffu;
                     float vfix = 1.f;
                     {
-                        const float4 b = *reinterpret_cast<const float4*>(sd.vbig[bar]);
-                        vfix = v_power(fmaxf(fmaxf(b.x, b.y), fmaxf(b.z, b.w)), vmost, vpow);
-                        if (vfix != 1.f) lpow = log2f(vpow);     // a power of two: exact
+                        const uint4 b = *reinterpret_cast<const uint4*>(sd.vbig[bar]);
+                        const uint4 s = *reinterpret_cast<const uint4*>(sd.vleast[bar]);
+                        vfix = v_power(__uint_as_float(max(max(b.x, b.y), max(b.z, b.w))), vmost, vpow);
+                        if (vfix != 1.f) lpow = exponent_of(vpow);
+                        vleast = min(min(vleast, min(s.x, s.y)), min(s.z, s.w));
                     }
                     // Lanes 0-15, then 16-31, by one piece of code (unrolled
                     // twice, it and the loaders' would not fit the instruction
@@ -810,6 +814,21 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
             have_o = have_o && alive;
             // log2 units; -inf: no key
             float m2 = m_used == -INFINITY ? -INFINITY : m_used * c - lpow;
+            if constexpr (Q8) {
+                if (have_o && wide_scales(vleast, vmost, vpow)) {
+                    float mx = 0.f;
+#pragma unroll 1
+                    for (int c0 = 0; c0 < D; c0 += 32) {
+                        uint32_t v[32];
+                        tmem_ld32(o_addr + c0, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) mx = fmaxf(mx, fabsf(__uint_as_float(v[i])));
+                    }
+                    if (m2 != -INFINITY && mx < trusted_from<ELEM, CT>(tnt * BKEY, vmost, vpow))
+                        m2 = __uint_as_float(0x7fffffffu);
+                }
+            }
             const bool split = sg.parts > 1;
             bool final = !split;
             Climb up(sg);
@@ -893,7 +912,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                     }
                 }
                 if (row_ok && a.lse) a.lse[pl.head * a.lh + pl.token] = lse_of(m2, l);
-                unsigned bad = __ballot_sync(0xffffffffu, row_ok && z != 0.f);
+                unsigned bad = __ballot_sync(0xffffffffu, row_ok && (z != 0.f || m2 != m2));
                 for (; bad; bad &= bad - 1) repair_row(a, sg, quarter * 32 + __ffs(bad) - 1);
             }
             __syncwarp();

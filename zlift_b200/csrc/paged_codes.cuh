@@ -70,22 +70,54 @@ struct Code<kBF16, kE4M3> {
     }
 };
 
-// fp16 weights carry a power of two `pow` beside the V scales, so that neither
-// a large scale (up to 516 times a weight of 64) overflows nor a small one
-// loses its bits to fp16's subnormals: pow * (largest scale seen) stays in
-// [1, 512].  Takes the largest scale of the next keys; returns the factor by
-// which the O summed so far has to be multiplied.
+// fp16 weights carry their keys' V scales and a power of two `pow`, by which
+// pow * (largest scale so far) stays in [128, 512]: a weight of 64 (the most
+// that a lazy maximum allows) does not overflow, and small scales keep their
+// bits as far down as fp16 goes.  Takes the largest scale of the next keys;
+// returns the factor by which the O summed so far has to be multiplied.
+// (Within 2^-90 and 2^90 the sums of 2^31 weights stay in fp32's range.)
 __device__ __forceinline__ float v_power(float big, float& most, float& pow) {
     if (!(big > most)) return 1.f;
     most = big;
     const float x = big * pow;
-    if (x >= 1.f && x <= 512.f) return 1.f;
-    // 2^-exponent(big), kept within what fp32 holds both ways
-    const int e = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 100);
-    const float next = __uint_as_float((uint32_t)(127 - e) << 23);
+    if (x >= 128.f && x <= 512.f) return 1.f;
+    const int e = min(max(134 - (int)(__float_as_uint(big) >> 23), -90), 90);
+    const float next = __uint_as_float((uint32_t)(127 + e) << 23);
     const float fix = next / pow;
     pow = next;
     return fix;
+}
+
+// log2 of a power of two
+__device__ __forceinline__ float exponent_of(float pow) {
+    return (float)((int)(__float_as_uint(pow) >> 23) - 127);
+}
+
+// A scale as a key for a maximum (`other` 0) or a minimum (all ones) over the
+// keys that count: those with a scale of zero, none or a NaN do not, nor do
+// infinities (which end in a NaN by themselves).
+__device__ __forceinline__ uint32_t scale_key(float s, uint32_t other) {
+    const uint32_t k = __float_as_uint(s) & 0x7fffffffu;
+    return k - 1u < 0x7f7fffffu ? k : other;
+}
+
+// `pow` is one number for all keys of a tile, hidden ones and ones without
+// weight among them, and a scale far below the largest leaves its weight
+// among fp16's subnormals.  Where s * pow >= 1 for every scale, no weight
+// loses more than an fp16 weight without a scale would.  Otherwise (`wide`) a row
+// is looked at by its result: each of the n weights is off by 2^-25 at most
+// beside its rounding, so O by n * 2^-25 * (largest code), and a row whose
+// largest |O| (with pow in it) is not well above that is computed again
+// (paged_finish.cuh) in fp32.
+__device__ __forceinline__ bool wide_scales(uint32_t least, float most, float pow) {
+    return __uint_as_float(least) * pow < 1.f || most * pow > 512.f;
+}
+// what the largest |O| must reach: the loss is then below half of what
+// rounding it to the output's type may cost
+template <int ELEM, int CT>
+__device__ __forceinline__ float trusted_from(int keys, float most, float pow) {
+    constexpr float per_key = (CT == kI8 ? 128.f : 448.f) * 0x1p-25f * (ELEM == kBF16 ? 0x1p9f : 0x1p12f);
+    return most * pow > 512.f ? INFINITY : keys * per_key;
 }
 
 }  // namespace zl

@@ -213,8 +213,8 @@ __device__ __forceinline__ void join_parts(const PagedAttn& a, const Segment& sg
 #pragma unroll 8
         for (int u = 0; u < c.members; u++) {
             const float4 ml = __ldcg(reinterpret_cast<const float4*>(slot(u)) + nb * 4 + t);
-            mm[0] = fmaxf(mm[0], ml.x);
-            mm[1] = fmaxf(mm[1], ml.z);
+            mm[0] = max_nan(mm[0], ml.x);
+            mm[1] = max_nan(mm[1], ml.z);
         }
         m[nb][0] = mm[0];
         m[nb][1] = mm[1];
@@ -243,6 +243,25 @@ __device__ __forceinline__ void join_parts(const PagedAttn& a, const Segment& sg
             }
         }
     }
+}
+
+// Rows whose largest |O| is below `from`: a maximum of NaN (paged_codes.cuh).
+template <int D, int NB>
+__device__ __forceinline__ void distrust_rows(const float (&o)[D / 16][NB][4], float (&m)[NB][2],
+                                              const float (&l)[NB][2], float from) {
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            float mx = 0.f;
+#pragma unroll
+            for (int j = 0; j < D / 16; j++)
+                mx = fmaxf(mx, fmaxf(fabsf(o[j][nb][e]), fabsf(o[j][nb][2 + e])));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            if (m[nb][e] != -INFINITY && mx < from) m[nb][e] = __uint_as_float(0x7fffffffu);
+        }
 }
 
 // Normalises and stores a tile's rows, and redoes those a masked key spoilt.
@@ -283,7 +302,7 @@ __device__ __forceinline__ void finish_rows(const PagedAttn& a, const Segment& s
                 }
             }
             if (live && g == 0 && a.lse) a.lse[pl.head * a.lh + pl.token] = lse_of(m[nb][e], l[nb][e]);
-            const unsigned bad = __ballot_sync(0xffffffffu, live && z != 0.f);
+            const unsigned bad = __ballot_sync(0xffffffffu, live && (z != 0.f || m[nb][e] != m[nb][e]));
             if (bad)
                 for (int i = 0; i < 4; i++)
                     if ((bad >> i) & 0x11111111u) repair_row(a, sg, nb * 8 + 2 * i + e);
@@ -478,6 +497,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
             l[nb][0] = l[nb][1] = 0.f;
         }
         float vmost = 0.f, vpow = 1.f, lpow = 0.f;   // 8 bit: see v_power
+        uint32_t vleast = 0xffffffffu;               // of this lane's keys
 
         for (int i = 0; i < mine; i++) {
             __syncwarp();                            // the stage to fill is no longer read
@@ -592,16 +612,16 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
                 }
             float vfix = 1.f;
             if constexpr (C::Q8) {
-                float big = 0.f;
-                if (C::BK >= 32 || lane < C::BK)
-                    big = __uint_as_float(lds4(sc + 16 + (C::BK + lane) * 4));
-                if (PL > 1)
-                    big = fmaxf(big, __uint_as_float(lds4(sc + 16 + (C::BK + 32 + lane) * 4)));
+                uint32_t big = 0;
 #pragma unroll
-                for (int o2 = 16; o2 > 0; o2 >>= 1)
-                    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o2));
-                vfix = v_power(big, vmost, vpow);
-                if (vfix != 1.f) lpow = log2f(vpow); // a power of two: exact
+                for (int h = 0; h < PL; h++)
+                    if (C::BK >= 32 || lane < C::BK) {
+                        const float s = __uint_as_float(lds4(sc + 16 + (C::BK + h * 32 + lane) * 4));
+                        big = max(big, scale_key(s, 0u));
+                        vleast = min(vleast, scale_key(s, 0xffffffffu));
+                    }
+                vfix = v_power(__uint_as_float(__reduce_max_sync(0xffffffffu, big)), vmost, vpow);
+                if (vfix != 1.f) lpow = exponent_of(vpow);
                 grow = grow || vfix != 1.f;
             }
             if (__any_sync(0xffffffffu, grow)) {
@@ -703,6 +723,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
                 l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], 16);
                 m[nb][e] -= lpow;                    // log2 units, of O and l alike
             }
+        if constexpr (C::Q8) {
+            if (wide_scales(__reduce_min_sync(0xffffffffu, vleast), vmost, vpow))
+                distrust_rows<D, NB>(o, m, l, trusted_from<ELEM, CT>(sg.k1 - sg.k0, vmost, vpow));
+        }
         bool final = sg.parts == 1;
         if (!final) store_part<D, NB>(part_slot(a, C::ROWS, piece, sg.part == 0), o, m, l);
         if (more) first_blocks(nx);

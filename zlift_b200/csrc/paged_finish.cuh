@@ -6,6 +6,8 @@
 // So every stored value is looked at, and a row with one that is not finite
 // is computed again by paged_row.cuh, which does not read the keys that the
 // row does not see.  Rows that are not finite by right come out the same.
+// Rows whose weights lost their bits (paged_codes.cuh) carry a maximum of NaN
+// and are computed again too.
 #pragma once
 #include "paged_row.cuh"
 #include "paged_sched.cuh"
@@ -23,6 +25,13 @@ __device__ __forceinline__ RowPlace row_place(const PagedAttn& a, const Segment&
 
 __device__ __forceinline__ float lse_of(float m2, float l) {
     return l == 0.f ? -INFINITY : m2 * 0.6931471805599453f + logf(l);
+}
+
+// the larger one, NaN if either is
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
 
 // by a warp
