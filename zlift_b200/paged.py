@@ -188,13 +188,15 @@ def kv_read(cache: KVCache, k_out, v_out, page_table, cu, starts=None, stream=No
                                 batch, 0 if stream is None else _stream(stream))
 
 
-_workspaces = {}
+_workspaces = {}        # (device, stream): the one that calls use now
+_outgrown = []          # those before it: captured graphs may still use them
 
 
 def _workspace(device: int, stream: int, nbytes: int):
     """The workspace of a device and stream: zeroed when made, replaced when a
-    call wants more.  Made on that stream, so an older one is reused only
-    after the work that still reads it."""
+    call wants more.  The old one stays allocated, since a graph captured with
+    it goes on using it (a stream needs a few sizes at most, some 100 MB in
+    all)."""
     on = torch.cuda.ExternalStream(stream, device=device) if stream else \
         torch.cuda.default_stream(device)
     with torch.cuda.stream(on):
@@ -202,6 +204,8 @@ def _workspace(device: int, stream: int, nbytes: int):
             raise RuntimeError("no workspace for this stream yet: call once before the capture, "
                                "or pass workspace=")
         ws = torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", device))
+    if (device, stream) in _workspaces:
+        _outgrown.append(_workspaces[(device, stream)])
     _workspaces[(device, stream)] = ws
     return ws
 
@@ -215,7 +219,10 @@ def paged_attention(cache: KVCache, q, o, lse, page_table, cu_q, seq_k, max_q, c
 
     workspace: a zeroed uint8 CUDA tensor of ``attention_workspace`` bytes
     that no concurrent call uses; by default one per device and stream is
-    kept (make one call outside a graph capture first, so that it exists).
+    kept for good (make one call outside a graph capture first, so that it
+    exists).  A captured graph goes on using the workspace of its capture, so
+    its replays and the calls on that stream must run one after another, or
+    the capture be given a workspace of its own.
     """
     device, kind, shape = cache.device, q.dtype, q.shape
     if len(shape) != 3 or shape != o.shape or o.dtype is not kind or shape[2] != cache.dim or \
