@@ -89,6 +89,8 @@ struct Side {
     uint32_t tmem;
     int abort;
     int last[2];
+    int ended[2][2];                 // of the partial unit that began before, begins here: tile joined here
+    int redo;                        // rows are marked in O
     alignas(16) uint32_t there[kMaxBars][4];     // which keys of the tile are in the cache
     alignas(16) uint32_t vbig[kMaxBars][4];      // 8 bit: largest V scale of 32 keys,
     alignas(16) uint32_t vleast[kMaxBars][4];    // and the smallest (scale_key)
@@ -231,6 +233,37 @@ __device__ __forceinline__ void join_columns(const PagedAttn& a, const Segment& 
     }
 }
 
+// by a thread, after it has stored row r
+static __device__ __noinline__ void mark_row(const PagedAttn& a, const Segment& g, int r, float m2, int* redo) {
+    const int end = (tile_end(a, g.q, g.i0 + g.ni) + BKEY - 1) / BKEY * BKEY;
+    const RowPlace p = row_place(a, g, r);
+    if (!redo_row(a, m2, keys_seen(a, g.q, p.token - g.q.q0), min(end, g.q.len))) return;
+    *reinterpret_cast<uint16_t*>(a.o + (p.token * a.orow + p.head * a.oh) * 2) = kRedo;
+    *redo = 1;
+}
+
+// Once a block's tiles are finished: its warps walk the piece again and compute
+// the marked rows of the tiles that it stored.
+static __device__ __noinline__ void redo_marked(const PagedAttn& a, const ChunkShape& c, const Side& sd) {
+    const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    Walker w;
+    w.start(a, c.sched, blockIdx.x);
+    Segment g;
+    while (w.next(a, c.sched, blockIdx.x, g)) {
+        const int i0 = g.i0, ni = g.ni;
+        for (int t = 0; t < 2; t++) {
+            if (g.parts > 1 && !sd.ended[g.part == 0][t]) continue;
+            g.i0 = i0 + t * c.tile_tokens;
+            g.ni = max(0, min(ni - t * c.tile_tokens, c.tile_tokens));
+            for (int r = warp; r < g.ni * a.group; r += warps) {
+                const RowPlace p = row_place(a, g, r);
+                const char* o = a.o + (p.token * a.orow + p.head * a.oh) * 2;
+                if (*reinterpret_cast<const volatile uint16_t*>(o) == kRedo) repair_row(a, g, r);
+            }
+        }
+    }
+}
+
 template <int D, int ELEM, int CT>
 __global__ void __launch_bounds__(PCfg<D, (CT >= kI8)>::THREADS, 1)
 paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
@@ -267,6 +300,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
             sd.pready[i] = 0;
         }
         sd.abort = 0;
+        sd.redo = 0;
+        for (int i = 0; i < 4; i++) sd.ended[i >> 1][i & 1] = 0;
         fence_mbar_init();
     }
     if (warp == C::MMA_WARP) {
@@ -912,8 +947,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                     }
                 }
                 if (row_ok && a.lse) a.lse[pl.head * a.lh + pl.token] = lse_of(m2, l);
-                unsigned bad = __ballot_sync(0xffffffffu, row_ok && (z != 0.f || m2 != m2));
-                for (; bad; bad &= bad - 1) repair_row(a, sg, quarter * 32 + __ffs(bad) - 1);
+                if (row_ok && spoilt(m2, l, z)) mark_row(a, sg, r, m2, &sd.redo);
+                if (split && r == 0) sd.ended[sg.part == 0][t] = 1;
             }
             __syncwarp();
         }
@@ -925,6 +960,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
         tc_fence_after();
         tmem_dealloc(tmem_base, 512);
     }
+    if (sd.redo && !sd.abort) redo_marked(a, shape, sd);
 }
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,

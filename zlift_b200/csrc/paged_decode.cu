@@ -271,6 +271,7 @@ __device__ __forceinline__ void finish_rows(const PagedAttn& a, const Segment& s
                                             const float (&l)[NB][2]) {
     using C = DCfg<D, CT, NB>;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int end = tile_end(a, sg.q, sg.i0 + sg.ni);
     const bool vec = ((reinterpret_cast<uintptr_t>(a.o) | (a.orow * 2) | (a.oh * 2)) & 15) == 0;
 #pragma unroll
     for (int nb = 0; nb < NB; nb++)
@@ -302,7 +303,9 @@ __device__ __forceinline__ void finish_rows(const PagedAttn& a, const Segment& s
                 }
             }
             if (live && g == 0 && a.lse) a.lse[pl.head * a.lh + pl.token] = lse_of(m[nb][e], l[nb][e]);
-            const unsigned bad = __ballot_sync(0xffffffffu, live && (z != 0.f || m[nb][e] != m[nb][e]));
+            const unsigned bad = __ballot_sync(
+                0xffffffffu, live && spoilt(m[nb][e], l[nb][e], z) &&
+                                redo_row(a, m[nb][e], keys_seen(a, sg.q, pl.token - sg.q.q0), end));
             if (bad)
                 for (int i = 0; i < 4; i++)
                     if ((bad >> i) & 0x11111111u) repair_row(a, sg, nb * 8 + 2 * i + e);
