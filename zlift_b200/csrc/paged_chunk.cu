@@ -1002,7 +1002,7 @@ int launch(const PagedAttn& a, cudaStream_t s) {
     using C = PCfg<D, (CT >= kI8)>;
     ChunkShape shape;
     shape.tile_tokens = BQ / a.group;
-    shape.sched = SchedShape{2 * shape.tile_tokens, BKEY, 2, chunk_blocks()};
+    shape.sched = sched_shape(a, 2 * shape.tile_tokens, BKEY, 2, chunk_blocks());
     shape.box = 8;
     while (shape.box < BKEY && a.c.ps % (2 * shape.box) == 0) shape.box *= 2;
     CUtensorMap tq, tk, tv;

@@ -841,7 +841,7 @@ int launch(const PagedAttn& a, cudaStream_t s) {
         attr_set.fetch_or(bit);
     }
     const int blocks = blocks_for(a);
-    const SchedShape shape{C::ROWS / a.group, C::BK, kLeast, blocks * kWarps};
+    const SchedShape shape = sched_shape(a, C::ROWS / a.group, C::BK, kLeast, blocks * kWarps);
     int box = 8;                                     // tokens of a page side by side
     while (box < C::BK && a.c.ps % (2 * box) == 0) box *= 2;
     CUtensorMap tk, tv;

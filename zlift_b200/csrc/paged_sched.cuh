@@ -7,8 +7,8 @@
 // each worker (a block, or a warp where warps work alone).  Lengths live on
 // the device, so every worker finds its piece from them: nothing is planned
 // on the host, a ragged batch is as even as a regular one, and a graph
-// replays with new lengths.  (Positions are 32 bits: 2^32 steps are minutes
-// of work.)
+// replays with new lengths.  Positions are 32 bits: where the work that the
+// arrays can hold would pass that, a step is several key tiles (sched_shape).
 //
 // A unit that spans several pieces is joined by whichever worker finishes
 // last: each leaves its unnormalised O with the maximum and the sum of every
@@ -28,6 +28,21 @@ struct SchedShape {
     int least;           // steps per piece, at least
     int pieces;
 };
+
+// Of tiles of `tokens` query tokens and `keys` keys.  A long chunk in tiles of
+// single tokens is 2^32 key tiles soon (131072 tokens, 16 keys, 8 heads), so
+// the step is doubled until the longest line that total_q, batch and the page
+// table's width allow is below 2^31 steps.
+inline SchedShape sched_shape(const PagedAttn& a, int tokens, int keys, int least, int pieces) {
+    SchedShape h{tokens, keys, least, pieces};
+    const double tiles = ((double)a.total_q / tokens + a.batch) * a.c.heads;
+    const double room = (double)a.tpages * a.c.ps;
+    while (h.step < (1 << 29) && tiles * (room / h.step + 2) >= 2147483648.0) {
+        h.step *= 2;
+        h.least = (h.least + 1) / 2;
+    }
+    return h;
+}
 
 // a unit, or what of it falls into one piece
 struct Segment {
