@@ -6,7 +6,8 @@
  * with a K/V cache (seqlen_knew) and ragged batches
  * (zblas/zblas_gpu.cpp:1424-1535).  These entries keep the manner of
  * zlift_attention.h: everything is enqueued on `stream` (0: the legacy
- * default stream) and nothing synchronises, allocates or copies to the host.
+ * default stream) of the current device, which has to be the operands', and
+ * nothing synchronises, allocates or copies to the host.
  *
  * Return value of every entry: 0 = done (enqueued), 1 = declined (the
  * arguments ask for something the kernels do not do; nothing was launched;

@@ -5,7 +5,8 @@
 ``paged_attention`` call the C entries with it.  Like the other attention
 calls they fill buffers that the caller made, run on ``stream`` (None: the
 legacy default stream, PyTorch's default) and return 0 done, 1 declined,
-2 launch failure.  Tensors whose shapes or types contradict each other raise
+2 launch failure.  Tensors whose shapes or types contradict each other, or
+whose GPU is not the current device (on which the C entries launch), raise
 ``ValueError``, which the C side could not see.
 """
 from __future__ import annotations
@@ -106,6 +107,11 @@ def _table(t, device):
     return shape[0], shape[1], stride
 
 
+def _on(device):
+    if torch.cuda.current_device() != device:
+        raise ValueError("the cache's GPU is not the current device")
+
+
 def _stream(stream) -> int:
     return 0 if stream is None else int(getattr(stream, "cuda_stream", stream))
 
@@ -159,6 +165,7 @@ class KVCache:
         vr, vh, v1 = v.stride()
         if (k1 != 1 or v1 != 1) and shape[2] > 1:
             raise ValueError("k and v: dim is not contiguous")
+        _on(device)
         return _rows_struct.pack(k.data_ptr(), v.data_ptr(), kr, kh, vr, vh, shape[0],
                                  _type(k)), shape[0]
 
@@ -243,6 +250,7 @@ def paged_attention(cache: KVCache, q, o, lse, page_table, cu_q, seq_k, max_q, c
                 (l1 != 1 and total > 1) or lse.get_device() != device:
             raise ValueError("lse: float32 [heads, total_q], total_q contiguous")
         lse_ptr = lse.data_ptr()
+    _on(device)
     lib, s = load(), 0 if stream is None else _stream(stream)
     ws = workspace if workspace is not None else _workspaces.get((device, s))
     while True:
