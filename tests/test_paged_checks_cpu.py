@@ -27,3 +27,16 @@ def test_another_current_device_is_refused(monkeypatch):
         paged.kv_read(cache, x, x, table, i32(0, 3))
     with pytest.raises(ValueError, match="current device"):
         paged.paged_attention(cache, q, q.clone(), None, table, i32(0, 3), i32(5), 3)
+
+
+def test_the_package_imports_without_torch():
+    """`import *` and the calls on plain pointers need no torch; the paged
+    calls are there by name where it is."""
+    code = ("import sys; sys.modules['torch'] = None\n"
+            "from zlift_b200 import *\n"
+            "assert Handle and flash_forward and load and 'kv_write' not in globals()\n")
+    subprocess.run([sys.executable, "-c", code], cwd=ROOT, check=True)
+    import zlift_b200
+    from zlift_b200 import KVCache, kv_read, kv_write, paged, paged_attention
+    assert zlift_b200.KVCache is KVCache is paged.KVCache
+    assert (kv_write, kv_read, paged_attention) == (paged.kv_write, paged.kv_read, paged.paged_attention)

@@ -129,7 +129,8 @@ from .attention import flash_forward, fmha_forward, FlashParams, FmhaParams  # n
 
 
 def __getattr__(name):
-    # the paged cache's calls need torch, which the rest of the package does not import
+    # the paged cache's calls need torch, which the rest of the package does not
+    # import: so they are not in __all__ either
     if name in ("KVCache", "kv_write", "kv_read", "paged_attention"):
         from . import paged
         return getattr(paged, name)
@@ -137,5 +138,4 @@ def __getattr__(name):
 
 
 __all__ = ["load", "Handle", "GemmError", "flash_forward", "fmha_forward",
-           "FlashParams", "FmhaParams", "KVCache", "kv_write", "kv_read", "paged_attention",
-           "LIBCUBLAS", "LIBCUDNN"]
+           "FlashParams", "FmhaParams", "LIBCUBLAS", "LIBCUDNN"]
