@@ -73,8 +73,10 @@ typedef struct zlift_kv_rows {
 } zlift_kv_rows;
 
 /* Writes token t's K and V rows into slot slots[t] (device, int32; a negative
- * slot skips the token, as padding needs it; two tokens with one slot leave
- * either).  rows->elem is F16 or BF16; a 16-bit cache has the same type.
+ * slot skips the token, as padding needs it; the others must differ: what two
+ * tokens leave in one slot is undefined, codes of one beside the scale of the
+ * other included).  rows->elem is F16 or BF16; a 16-bit cache has the same
+ * type.
  *
  * An 8-bit row x is stored as scale = amax / top and codes
  * round(x * (top / amax)), amax = max |x|, top = 127 (I8) or 448 (E4M3);

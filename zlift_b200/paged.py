@@ -172,7 +172,7 @@ class KVCache:
 
 def kv_write(cache: KVCache, k, v, slots, stream=None) -> int:
     """Writes packed k, v [tokens, heads, dim] into slots [tokens] (int32:
-    page * page_size + offset; negative: skipped)."""
+    page * page_size + offset; negative: skipped; otherwise no two alike)."""
     rows, tokens = cache._rows(k, v)
     if _index(slots, cache.device, "slots") != tokens:
         raise ValueError("one slot for each token")
