@@ -22,6 +22,14 @@ static __device__ __noinline__ void note_bad_index() {
     atomicCAS(&g_dev_error, 0, kErrBadIndex);
 }
 
+// Waits for copies or products that are under way, whoever has given up
+// (bounded too, by the default limit: a shorter one that was set is for waits
+// on other parts of a kernel).
+__device__ __forceinline__ void copy_wait(uint64_t* bar, uint32_t parity) {
+    volatile int never = 0;
+    mbar_wait_for(bar, parity, &never, kDefaultWaitLimitNs);
+}
+
 // n / d for 0 <= n < 2^31, d >= 1: one multiply-high and a shift.  With
 // s = ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1 the quotient is
 // (mulhi(m, n) + n) >> s (Granlund and Montgomery 1994, figure 4.1); the sum

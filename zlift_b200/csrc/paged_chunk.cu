@@ -82,7 +82,7 @@ constexpr int kMaxBars = 5;          // KV_BARS at most (NSLOT 8)
 // what sits behind the tiles in shared memory
 struct Side {
     uint64_t qfull, qempty, vtail;
-    uint64_t sfull[2], ofinal[2];
+    uint64_t sfull[2], ofinal[2], drained;
     uint64_t kvfull[kMaxBars];
     uint64_t kvempty[8];
     uint32_t pready[2];              // softmax -> MMA: warps done, 4 per key tile
@@ -290,7 +290,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
         mbar_init(&sd.qfull, 1);
         mbar_init(&sd.qempty, 1);
         mbar_init(&sd.vtail, 1);
-        // 16 bit: the byte count's arrival, and "the tile is as it shall be";
+        mbar_init(&sd.drained, 1);
+        // 16 bit: one arrival for K and one for V, each with its byte count (a V
+        // tile that had to be cleaned: once it is);
         // 8 bit: each loader warp, once for K and once for V
         for (int i = 0; i < KV_BARS; i++) mbar_init(&sd.kvfull[i], Q8 ? 2 * C::LOADERS : 2);
         for (int i = 0; i < NSLOT; i++) mbar_init(&sd.kvempty[i], 1);
@@ -321,6 +323,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
     if (warp >= 8 && warp < C::MMA_WARP) {
         // ---------------- loaders ----------------
         uint32_t step = 0, segs = 0, tails = 0;      // key tiles, segments, cleaned tails so far
+        uint32_t asked = 0, asked_q = 0;             // key tiles and Q tiles on their way or here
         bool ok = true;
         Segment sg;
         // (8 bit: a warp that gave up goes on through the named barriers that
@@ -331,6 +334,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
             if (warp == 8 && ok) {
                 if (segs > 0) ok = mbar_wait(&sd.qempty, (segs - 1) & 1, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
+                asked_q += ok;
                 if (ok && lane == 0) {
                     // the box clips nothing but the end of q, and counts its
                     // bytes there too
@@ -372,11 +376,12 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                         const uint32_t item = 2 * step + kv, slot = item % NSLOT;
                         ok = mbar_wait(&sd.kvempty[slot], ((item / NSLOT) & 1) ^ 1u, abort_flag);
                         ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) break;
-                        if (lane == 0) {
-                            if (kv == 0) mbar_expect_tx(full, (tail ? 1 : 2) * C::TILE_BYTES);
-                            else if (tail) mbar_expect_tx(&sd.vtail, C::TILE_BYTES);
+                        if (!ok) {                   // (K's phase shall end with its bytes)
+                            if (kv && lane == 0) mbar_arrive(full);
+                            break;
                         }
+                        asked = step + 1;
+                        if (lane == 0) mbar_expect_tx(kv && tail ? &sd.vtail : full, C::TILE_BYTES);
                         if (kv == 0 && lane < 4) {
                             uint32_t w = 0xffffffffu;
                             if (gone)
@@ -392,7 +397,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                         if (kv && tail) {
                             ok = mbar_wait(&sd.vtail, tails & 1, abort_flag);
                             ok = __all_sync(0xffffffffu, ok);
-                            if (!ok) break;
+                            if (!ok) {
+                                if (lane == 0) {
+                                    copy_wait(&sd.vtail, tails & 1);
+                                    mbar_arrive(full);
+                                }
+                                break;
+                            }
                             tails++;
                             const int end = (left + box - 1) / box * box;
                             constexpr int PIECES = 8 * C::BOXES;
@@ -403,9 +414,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                             }
                             fence_async_smem();
                             __syncwarp();
+                            if (lane == 0) mbar_arrive(full);
                         }
                     }
-                    if (ok && lane == 0) mbar_arrive(full);
                 }
             } else {
                 constexpr int CPR = D / 16;          // 16-byte pieces of a row
@@ -510,7 +521,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
             const uint32_t items = 2 * step;
             for (uint32_t i = items > NSLOT ? items - NSLOT : 0; ok && i < items; i++)
                 ok = mbar_wait(&sd.kvempty[i % NSLOT], (i / NSLOT) & 1, abort_flag);
-            if (ok) mbar_wait(&sd.qempty, (segs - 1) & 1, abort_flag);
+            ok = ok && mbar_wait(&sd.qempty, (segs - 1) & 1, abort_flag);
+        }
+        // gave up: not before the copies have landed
+        if (warp == 8 && lane == 0 && !ok) {
+            if (asked_q > 0) copy_wait(&sd.qfull, (asked_q - 1) & 1);
+            for (uint32_t j = asked > KV_BARS ? asked - KV_BARS : 0; j < asked; j++)
+                copy_wait(&sd.kvfull[j % KV_BARS], (j / KV_BARS) & 1);
         }
     } else if (warp == C::MMA_WARP) {
         // ---------------- MMA issuer ----------------
@@ -586,6 +603,12 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
             ok = __shfl_sync(0xffffffffu, ok, 0);
             step += sp.nmax;
             segs++;
+        }
+        // whatever the other roles have waited for: no product and no commit
+        // outlives the block
+        if (lane == 0) {
+            mma_commit(&sd.drained);
+            copy_wait(&sd.drained, 0);
         }
     } else {
         // ---------------- softmax and epilogue (warps 0-7) ----------------

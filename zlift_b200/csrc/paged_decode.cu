@@ -758,9 +758,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
         sg = nx;
     }
     if (!alive) {                                    // gave up: not before the copies have landed
-        volatile int never = 0;
-        for (; in_flight > 0; in_flight--, out.next(stages))
-            mbar_wait_for(&s_full[warp][out.at], out.phase, &never, g_wait_limit_ns);
+        for (; in_flight > 0; in_flight--, out.next(stages)) copy_wait(&s_full[warp][out.at], out.phase);
     }
 }
 
