@@ -233,6 +233,22 @@ __device__ __forceinline__ void join_columns(const PagedAttn& a, const Segment& 
     }
 }
 
+// The row's maximum, or NaN where its largest |O| is below `from`
+// (paged_codes.cuh).
+template <int D>
+static __device__ __noinline__ float trusted_max(uint32_t o_addr, float m2, float from) {
+    float mx = 0.f;
+#pragma unroll 1
+    for (int c0 = 0; c0 < D; c0 += 32) {
+        uint32_t v[32];
+        tmem_ld32(o_addr + c0, v);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; i++) mx = fmaxf(mx, fabsf(__uint_as_float(v[i])));
+    }
+    return m2 != -INFINITY && mx < from ? __uint_as_float(0x7fffffffu) : m2;
+}
+
 // by a thread, after it has stored row r
 static __device__ __noinline__ void mark_row(const PagedAttn& a, const Segment& g, int r, float m2, int* redo) {
     const int end = (tile_end(a, g.q, g.i0 + g.ni) + BKEY - 1) / BKEY * BKEY;
@@ -740,9 +756,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                     float vfix = 1.f;
                     {
                         const uint4 b = *reinterpret_cast<const uint4*>(sd.vbig[bar]);
-                        const uint4 s = *reinterpret_cast<const uint4*>(sd.vleast[bar]);
                         vfix = v_power(__uint_as_float(max(max(b.x, b.y), max(b.z, b.w))), vmost, vpow);
                         if (vfix != 1.f) lpow = exponent_of(vpow);
+                        const uint4 s = *reinterpret_cast<const uint4*>(sd.vleast[bar]);
                         vleast = min(min(vleast, min(s.x, s.y)), min(s.z, s.w));
                     }
                     // Lanes 0-15, then 16-31, by one piece of code (unrolled
@@ -873,19 +889,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
             // log2 units; -inf: no key
             float m2 = m_used == -INFINITY ? -INFINITY : m_used * c - lpow;
             if constexpr (Q8) {
-                if (have_o && wide_scales(vleast, vmost, vpow)) {
-                    float mx = 0.f;
-#pragma unroll 1
-                    for (int c0 = 0; c0 < D; c0 += 32) {
-                        uint32_t v[32];
-                        tmem_ld32(o_addr + c0, v);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 32; i++) mx = fmaxf(mx, fabsf(__uint_as_float(v[i])));
-                    }
-                    if (m2 != -INFINITY && mx < trusted_from<ELEM, CT>(tnt * BKEY, vmost, vpow))
-                        m2 = __uint_as_float(0x7fffffffu);
-                }
+                if (have_o && wide_scales(vleast, vmost, vpow))
+                    m2 = trusted_max<D>(o_addr, m2, trusted_from<ELEM, CT>(tnt * BKEY, vmost, vpow));
             }
             const bool split = sg.parts > 1;
             bool final = !split;
