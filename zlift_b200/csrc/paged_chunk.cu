@@ -634,8 +634,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
         const uint32_t s_addr = tmem_base + lane_off + (t ? C::S_COL1 : C::S_COL0);
         const uint32_t o_addr = tmem_base + lane_off + (t ? C::O_COL1 : C::O_COL0);
         const float c = Q8 ? 1.f : a.scale * kLog2e;     // 8 bit: in the K scales already
-        // weights reach 2^lazy; in fp16 times a V scale of up to 512
-        constexpr float kLazyLog2 = Q8 ? 6.f : 8.f;
+        constexpr float kLazyLog2 = Q8 ? kLazy8 : 8.f;   // weights reach 2^this
         uint32_t step = 0, tiles = 0, finals = 0;
         bool alive = true;
         Segment sg;

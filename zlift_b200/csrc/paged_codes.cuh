@@ -71,17 +71,24 @@ struct Code<kBF16, kE4M3> {
 };
 
 // fp16 weights carry their keys' V scales and a power of two `pow`, by which
-// pow * (largest scale so far) stays in [128, 512]: a weight of 64 (the most
-// that a lazy maximum allows) does not overflow, and small scales keep their
-// bits as far down as fp16 goes.  Takes the largest scale of the next keys;
-// returns the factor by which the O summed so far has to be multiplied.
-// (Within 2^-90 and 2^90 the sums of 2^31 weights stay in fp32's range.)
+// pow * (largest scale so far) stays in [256, 1024]: a weight of 2^kLazy8 (the
+// most that a lazy maximum allows) does not overflow, and small scales keep
+// their bits as far down as fp16 goes.
+//
+// A lazy maximum of 6 with [128, 512] took 587 us where this takes 594 (4 x 2048
+// over 4096 tokens, int8), but sent rows whose weight sits on one token with a V
+// 1000 times below the largest to be computed again (29 ms in place of 0.6).
+constexpr float kLazy8 = 5.f;
+
+// Takes the largest scale of the next keys; returns the factor by which the O
+// summed so far has to be multiplied.  (Within 2^-90 and 2^90 the sums of 2^31
+// weights stay in fp32's range.)
 __device__ __forceinline__ float v_power(float big, float& most, float& pow) {
     if (!(big > most)) return 1.f;
     most = big;
     const float x = big * pow;
-    if (x >= 128.f && x <= 512.f) return 1.f;
-    const int e = min(max(134 - (int)(__float_as_uint(big) >> 23), -90), 90);
+    if (x >= 256.f && x <= 1024.f) return 1.f;
+    const int e = min(max(135 - (int)(__float_as_uint(big) >> 23), -90), 90);
     const float next = __uint_as_float((uint32_t)(127 + e) << 23);
     const float fix = next / pow;
     pow = next;
@@ -110,14 +117,14 @@ __device__ __forceinline__ uint32_t scale_key(float s, uint32_t other) {
 // largest |O| (with pow in it) is not well above that is computed again
 // (paged_finish.cuh) in fp32.
 __device__ __forceinline__ bool wide_scales(uint32_t least, float most, float pow) {
-    return __uint_as_float(least) * pow < 1.f || most * pow > 512.f;
+    return __uint_as_float(least) * pow < 1.f || most * pow > 1024.f;
 }
-// what the largest |O| must reach: the loss is then below half of what
-// rounding it to the output's type may cost
+// what the largest |O| must reach: the loss is then below what rounding it to
+// the output's type may cost
 template <int ELEM, int CT>
 __device__ __forceinline__ float trusted_from(int keys, float most, float pow) {
-    constexpr float per_key = (CT == kI8 ? 128.f : 448.f) * 0x1p-25f * (ELEM == kBF16 ? 0x1p9f : 0x1p12f);
-    return most * pow > 512.f ? INFINITY : keys * per_key;
+    constexpr float per_key = (CT == kI8 ? 128.f : 448.f) * 0x1p-25f * (ELEM == kBF16 ? 0x1p8f : 0x1p11f);
+    return most * pow > 1024.f ? INFINITY : keys * per_key;
 }
 
 }  // namespace zl

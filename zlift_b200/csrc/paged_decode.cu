@@ -31,7 +31,7 @@
 //
 // Softmax in log2 units: x = s * scale * log2(e) (* K scale), weights
 // ex2(x - m) rounded to the 16-bit type for the product, summed unrounded in
-// fp32.  m is the running maximum, or up to 2^kLazy below it: O and l are
+// fp32.  m is the running maximum, or up to kLazy (kLazy8) below it: O and l are
 // rescaled only when it grew by more, and both carry the same m, so the
 // quotient does not change.  In fp16 a V scale could leave the type's range:
 // see v_power.
@@ -159,8 +159,9 @@ __device__ __forceinline__ uint32_t lds4(uint32_t a) {
 // Row block nb of the query operand from bf16 to fp16, the type that codes
 // widen to most cheaply and weights keep most bits in.  A row is brought to a
 // maximum of [1, 2) by a power of two (returned: its inverse): bf16's 8 bits fit
-// fp16's 11, and what lies 2^14 below the row's maximum and loses bits to
-// fp16's subnormals is off by 2^-25 of that maximum, as fp32 sums are.
+// fp16's 11, and what lies more than 2^17 below the row's maximum and loses bits
+// to fp16's subnormals is off by 2^-25 of that maximum (K's codes are off by
+// 2^-8 of theirs).
 template <int D, int NB>
 __device__ __forceinline__ float halve_row(uint32_t (&qb)[D / 16][NB][2], int nb) {
     unsigned most = 0;
@@ -607,7 +608,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
                     alpha[nb][e] = 1.f;
-                    if (mx > m[nb][e] + kLazy) {     // also from -inf
+                    if (mx > m[nb][e] + (C::Q8 ? kLazy8 : kLazy)) {     // also from -inf
                         alpha[nb][e] = ex2(m[nb][e] - mx);
                         m[nb][e] = mx;
                         grow = true;
