@@ -14,7 +14,7 @@
 // Measured on one B200, 8 heads of 128: reading 131072 int8 tokens back in bf16
 // 129 us, 6.3 TB/s, 96% of the copy rate; writing 8 x 4096 bf16 tokens to e4m3
 // 55 us, 3.7 TB/s (what is left is issue: a maximum, two quotients and eight
-// conversions per 16 bytes); 64 tokens written to int8 and read back 5.8 us,
+// conversions per 16 bytes); 64 tokens written to int8 and read back 6 us,
 // two launches.
 #include "gemm.h"
 #include "paged.h"

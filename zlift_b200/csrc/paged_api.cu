@@ -109,8 +109,14 @@ Way choose(const PagedAttn& a) {
                        a.group <= 128 && (reinterpret_cast<uintptr_t>(a.o) & 15u) == 0 &&
                        (a.orow * 2) % 16 == 0 && (a.oh * 2) % 16 == 0;
     // Few rows go to the kernel that reads the cache once for 24 of them; more,
-    // to the one with tiles of 128 rows.  20 rows (5 tokens, group 4, 32 x up to
-    // 4096 e4m3 tokens) took 80 us in the first and 320 us in the second.
+    // to the one with tiles of 128 rows.  Over 32 x up to 4096 tokens, dim 128, 8 KV
+    // heads, in us:
+    //              bf16 cache                e4m3 cache
+    //   rows   4   24   32   48  128     4   24   32   64  128
+    //   few   70   84   88  132  274    56   77   82  151  228   (from 32 on: one
+    //   tiles 101  105  101  113  116   174  177  173  199  179    read per 24 rows)
+    // So the tiles win from some 40 rows on over 16 bits and from some 80 over 8.
+    // The limit is the rows of one tile all the same.
     const long long rows = (long long)(a.max_q > 1 ? a.max_q : 1) * a.group;
     if (a.group <= decode_max_rows() && (rows <= decode_max_rows() || !boxes)) return Way::Decode;
     return boxes ? Way::Chunk : Way::Simt;

@@ -29,16 +29,18 @@
 //           layout that the tensor core reads; K of the next tile is on its
 //           way while V of this one is widened, and the other way round.  The
 //           K scale of a key multiplies its column of S and the V scale its
-//           column of P, so nothing is rounded that a 16-bit cache would not
-//           round.
+//           column of P, which is fp16 (what that loses where the scales lie
+//           far apart: paged_codes.cuh).
 //
 // Measured on one B200 (32/8 heads of 128): 512 new tokens over 32768, bf16,
-// 293 us in short runs (930 TFLOP/s), 344 us at the power cap; 4 ragged chunks
-// of up to 2048 over up to 4096 tokens, bf16 360 us, int8 565 us.  What 8 bits
-// cost there: instruction issue.  Three loader warps in place of six took 842
-// us; unrolling the softmax for both halves of a warp's rows 646 us, because
-// that code and the loaders' then overflow the instruction cache; a row of
-// scores per thread, whose 128 scales every thread reads, 760 us.
+// 295 us in short runs (925 TFLOP/s), 345 us at the power cap; 4 ragged chunks
+// of up to 2048 over up to 4096 tokens, bf16 366 us, int8 594 us, e4m3 590 us.
+// What 8 bits cost there: the loaders' and the softmax's instructions share the
+// issue slots (45% used, 0.65 of 8.4 warps waiting for instructions) and 128
+// registers a thread, with some 190 bytes of spills.  Earlier forms, when this
+// one took 565 us: three loader warps in place of six 842 us; the softmax
+// unrolled for both halves of a warp's rows 646 us; a row of scores per thread,
+// whose 128 scales every thread reads, 760 us.
 //
 // Roles (warps): 0-3 and 4-7 softmax of tile 0 and 1, then the loaders (one
 // or six), then the MMA issuer.

@@ -37,16 +37,16 @@
 // see v_power.
 //
 // Measured on one B200 (32 query and 8 KV heads of 128 unless said otherwise):
-// 64 ragged sequences of up to 4096 bf16 tokens 124 us, 5.5 TB/s, 84% of the
-// copy rate; while all warps run it moves 6.4 TB/s, and the rest is that some
-// SMs get less of the memory than others and end 15% later.  Handing the last
-// 15 to 30% of the keys out in small pieces to whoever was free cost more in
-// parts to join than it gained (145 us and up).  16 x 32768 int8 176 us, 3.9
-// TB/s: per block of codes a warp issues some 600 instructions, half of them
-// widening, in one dependent chain.  32 sequences of up to 4096 e4m3 tokens with
-// 5 drafted ones 80 us (20 rows, three row blocks); 16 heads of 64, e4m3, 24 x
-// up to 2047 tokens 29 us; one bf16 sequence of 515 tokens, 8/2 heads 13 us,
-// all of it latency (launch, look-ups, first bytes, blocks, join).
+// 64 ragged sequences of up to 4096 bf16 tokens 125 us, 5.5 TB/s, 84% of the
+// copy rate, every byte read from DRAM once.  Handing the last 15 to 30% of the
+// keys out in small pieces to whoever was free cost more in parts to join than
+// it gained (145 us and up).  16 x 32768 int8 175 us, 3.9 TB/s of codes and
+// scales: some 790 warp instructions per block of 8 KB, at 43% of the issue
+// slots, and DRAM reads 1.35 times the bytes (5.3 TB/s).  32 sequences of up to
+// 4096 e4m3 tokens with 5 drafted ones 80 us (20 rows, three row blocks); 16
+// heads of 64, e4m3, 24 x up to 2047 tokens 30 us; one bf16 sequence of 515
+// tokens, 8/2 heads 13.6 us, all of it latency (launch, look-ups, first bytes,
+// blocks, join).
 #include "gemm.h"
 #include "paged_codes.cuh"
 #include "paged_finish.cuh"
