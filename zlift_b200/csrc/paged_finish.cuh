@@ -61,7 +61,9 @@ static __device__ __noinline__ void repair_row(const PagedAttn& a, const Segment
     const int seen = keys_seen(a, g.q, p.token - g.q.q0);
     RowState r;
     r.clear();
+    __syncwarp();                                    // what the other lanes stored of it comes first
     row_keys(a, g.s, a.q + (p.token * a.qr + p.head * a.qh) * 2, g.head, 0, seen, 32, r);
     row_store(a, p.token, p.head, r);
 }
+
 }  // namespace zl
